@@ -274,6 +274,67 @@ int wfd_gather_pack(const void* k_cache, const void* v_cache, void* k_pack, void
                     void* stream);
 
 /* ---------------------------------------------------------------------------
+ * 8-bit KV-slot cache (no counterpart in the reference, whose cache holds the
+ * model's own type).  A cached row (one slot, sequence, position and kv head;
+ * head_dim values of K or V) is head_dim e4m3 codes q_i and one exponent e:
+ *   e = clamp(smallest integer with max |x_i| <= 448 * 2^e, -32, 32)
+ *   q_i = e4m3(x_i * 2^-e), nearest even, saturating;  value q_i * 2^e
+ * (a row of zeros has e = -32; an infinity has e = 32 and saturates; a NaN is
+ * stored as 0 and sets bit 256 of the error word).  head_dim a power of two, 16
+ * to 256; at most 1024 kv heads.  Rows are bf16 or f32 (dtype).
+ * ------------------------------------------------------------------------- */
+typedef struct wfd_q8_cache {
+  void* k;           /* (n_slots, n_seqs, max_seq, n_kv_heads, head_dim) e4m3 codes, 16-byte aligned */
+  void* v;
+  int8_t* k_exp;     /* (n_slots, n_seqs, n_kv_heads, max_seq) exponents                              */
+  int8_t* v_exp;
+  int32_t* lens;     /* (n_slots, n_seqs) slot lengths, or NULL                                       */
+  int32_t n_slots, n_seqs, max_seq, n_kv_heads, head_dim;
+} wfd_q8_cache;
+
+/* sizeof(wfd_q8_cache) as compiled into the library. */
+size_t wfd_q8_cache_bytes(void);
+
+/* wfd_append into an 8-bit cache.  At most WFD_Q8_MAX_APPEND rows a call; where
+ * several rows of a call name one place, the last of them is stored. */
+#define WFD_Q8_MAX_APPEND 16384
+int wfd_append_q8(const wfd_q8_cache* cache, const void* k_new, const void* v_new, const int32_t* slots,
+                  const int32_t* seqs, const int32_t* positions, int32_t n, int32_t slot_offset, int32_t dtype,
+                  int32_t* d_err, void* stream);
+
+/* wfd_write_prefill into an 8-bit cache (n_seqs <= 65535). */
+int wfd_write_prefill_q8(const wfd_q8_cache* cache, const void* k, const void* v, int32_t slot, int32_t L,
+                         int32_t dtype, int32_t* d_err, void* stream);
+
+/* Read back: segment i (of n <= 65535) writes the values of positions
+ * [0, cu_k[i+1] - cu_k[i]) of (slots[i], seqs[i]) to rows cu_k[i].. of k_pack /
+ * v_pack (total rows of (n_kv_heads, head_dim), `dtype`).  Segments that leave
+ * the cache or the packs are skipped and reported. */
+int wfd_gather_q8(const wfd_q8_cache* cache, void* k_pack, void* v_pack, const int32_t* slots, const int32_t* seqs,
+                  const int32_t* cu_k, int32_t n, int64_t total, int32_t dtype, int32_t* d_err, void* stream);
+
+/* wfd_commit_window for an 8-bit cache. */
+int wfd_commit_window_q8(const wfd_q8_cache* cache, const wfd_item* items, int32_t n_items, const int32_t* accept_len,
+                         const uint8_t* accept_mask, int32_t* acc_rows, int32_t* acc_count, int32_t n_rows,
+                         int32_t slot_offset, int32_t* d_err, void* stream);
+
+/* wfd_wave_attn over an 8-bit cache: the window rows are quantised into the
+ * cache, then every row attends the values the cache holds, its own included.
+ * q / out and k_new / v_new are `dtype` (bf16 or f32); head_dim 64 or 128; max_q an
+ * upper bound of the items' q_len (a longer item is reported).  row_pos as in
+ * wfd_wave_attn_rows, for either kernel.  which: -1 auto, 0 CUDA cores, 1 tcgen05
+ * (bf16; n_kv_heads * head_dim a multiple of 128).  scale 0 selects
+ * 1/sqrt(head_dim); a negative one is refused.  Where two items hold one position of a
+ * (slot, sequence), the later item's row is stored.  The workspace
+ * (wfd_wave_attn_q8_workspace bytes, 16-byte aligned) need not be initialised
+ * and holds nothing between calls: calls that may overlap each need their own. */
+size_t wfd_wave_attn_q8_workspace(int32_t n_items);
+int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const void* q, const void* k_new, const void* v_new,
+                     void* out, const wfd_item* items, int32_t n_items, int32_t max_q, const int32_t* row_pos,
+                     int32_t row_pos_stride, int32_t slot_offset, int32_t n_rows, int32_t n_heads, int32_t dtype,
+                     float scale, void* workspace, size_t workspace_bytes, int32_t* d_err, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Looped-LM block helpers used by the wavefront engine around the attention
  * (fused element-wise work of one transformer block; fp32 arithmetic, bf16 or
  * f32 storage).  The reference runs these as framework modules (norm, RoPE in

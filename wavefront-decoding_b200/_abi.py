@@ -29,7 +29,10 @@ EXPORTED = (
     "wfd_sched_pre_tick", "wfd_sched_route", "wfd_sched_settle", "wfd_sched_params_bytes",
     "wfd_set_batch_invariant", "wfd_get_batch_invariant", "wfd_test_fail_waits",
     "wfd_linear", "wfd_linear_params_bytes", "wfd_rope_split_norm", "wfd_silu_mul_norm",
+    "wfd_q8_cache_bytes", "wfd_append_q8", "wfd_write_prefill_q8", "wfd_gather_q8", "wfd_commit_window_q8",
+    "wfd_wave_attn_q8", "wfd_wave_attn_q8_workspace",
 )
+WFD_Q8_MAX_APPEND = 16384
 
 WFD_LINEAR_PLAIN, WFD_LINEAR_RESIDUAL, WFD_LINEAR_SWIGLU, WFD_LINEAR_ROPE = 0, 1, 2, 3
 
@@ -70,10 +73,17 @@ class wfd_linear_params(ctypes.Structure):
         [(n, ctypes.c_int32) for n in ("H", "Hkv", "Dh", "rope_style", "pos_stride", "pos_period", "max_pos")]
 
 
+class wfd_q8_cache(ctypes.Structure):
+    """include/wfd_b200.h: wfd_q8_cache (field order and types must match)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_exp", "v_exp", "lens")] + \
+        [(n, ctypes.c_int32) for n in ("n_slots", "n_seqs", "max_seq", "n_kv_heads", "head_dim")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+_L = ctypes.c_int64
 
 _SIGS = {
     "wfd_abi_version": ([], _I),
@@ -133,6 +143,18 @@ _SIGS = {
     # const wfd_linear_params*, stream
     "wfd_linear": ([_P, _P], _I),
     "wfd_linear_params_bytes": ([], _S),
+    "wfd_q8_cache_bytes": ([], _S),
+    # const wfd_q8_cache*, k_new v_new slots seqs positions n slot_off dtype err stream
+    "wfd_append_q8": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P], _I),
+    # cache k v slot L dtype err stream
+    "wfd_write_prefill_q8": ([_P, _P, _P, _I, _I, _I, _P, _P], _I),
+    # cache kp vp slots seqs cu_k n total dtype err stream
+    "wfd_gather_q8": ([_P, _P, _P, _P, _P, _P, _I, _L, _I, _P, _P], _I),
+    # cache items n accept_len accept_mask acc_rows acc_count n_rows slot_off err stream
+    "wfd_commit_window_q8": ([_P, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P], _I),
+    "wfd_wave_attn_q8_workspace": ([_I], _S),
+    # which cache q k_new v_new out items n max_q row_pos rp_stride slot_off n_rows Hq dtype scale ws ws_bytes err stream
+    "wfd_wave_attn_q8": ([_I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _F, _P, _S, _P, _P], _I),
     # const wfd_sched_params*, stream
     "wfd_sched_pre_tick": ([_P, _P], _I),
     "wfd_sched_route": ([_P, _P], _I),

@@ -20,6 +20,9 @@
 #include "wfd_sched.cuh"
 #include "wfd_plan.cuh"
 #include "wfd_prefill.cuh"
+#include "wfd_q8.cuh"
+#include "wfd_q8_attn.cuh"
+#include "wfd_q8_tc.cuh"
 #include "wfd_verify.cuh"
 
 using namespace wfd;
@@ -376,7 +379,7 @@ int run_attention(const AttnArgs& A, cudaStream_t st) {
     pp.lens_offset = A.slot_offset * A.n_seqs;
     plan_blocks = 1 + (A.n < 4 * sms ? A.n : 4 * sms);
   }
-  if (launch_pdl(plan_kernel, dim3(plan_blocks), dim3(kPlanThreads), 0, st, pp) != cudaSuccess)
+  if (launch_pdl(plan_kernel<void>, dim3(plan_blocks), dim3(kPlanThreads), 0, st, pp) != cudaSuccess)
     return WFD_ERR_CUDA;
 
   const float scale = A.scale > 0.f ? A.scale : 1.0f / std::sqrt((float)A.Dh);
@@ -1324,3 +1327,309 @@ extern "C" int wfd_sched_settle(const wfd_sched_params* p, void* stream) {
   return cudaGetLastError() == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
 }
 
+
+// ---------------------------------------------------------------------------
+// 8-bit KV-slot cache
+// ---------------------------------------------------------------------------
+namespace {
+
+// Host checks of an 8-bit cache and its device form, counted from slot_offset.
+int q8_cache(const wfd_q8_cache* c, int slot_offset, Q8Cache* out) {
+  if (!c || !c->k || !c->v || !c->k_exp || !c->v_exp) return WFD_ERR_INVALID_ARG;
+  if (c->n_slots <= 0 || c->n_seqs <= 0 || c->max_seq <= 0 || c->n_kv_heads <= 0) return WFD_ERR_INVALID_ARG;
+  if (slot_offset < 0 || slot_offset >= c->n_slots) return WFD_ERR_INVALID_ARG;
+  const int Dh = c->head_dim;
+  if (Dh < 16 || Dh > 256 || (Dh & (Dh - 1)) != 0 || c->n_kv_heads > kQ8MaxHeads) return WFD_ERR_UNSUPPORTED;
+  if (!aligned16(c->k) || !aligned16(c->v)) return WFD_ERR_ALIGNMENT;
+  const long long rows = (long long)slot_offset * c->n_seqs * c->max_seq;
+  out->k = static_cast<uint8_t*>(c->k) + rows * c->n_kv_heads * Dh;
+  out->v = static_cast<uint8_t*>(c->v) + rows * c->n_kv_heads * Dh;
+  out->ke = c->k_exp + rows * c->n_kv_heads;
+  out->ve = c->v_exp + rows * c->n_kv_heads;
+  out->n_slots = c->n_slots - slot_offset;
+  out->n_seqs = c->n_seqs;
+  out->max_seq = c->max_seq;
+  out->Hkv = c->n_kv_heads;
+  out->Dh = Dh;
+  return WFD_OK;
+}
+
+// (128 bytes, heads of 128 bytes, rows) view of a code buffer; box 128 bytes x 1 x
+// box_rows, 128-byte swizzle.
+bool make_q8_map(CUtensorMap* m, const void* base, long long rows, int row_bytes, int box_rows) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {128, (cuuint64_t)(row_bytes / 128), (cuuint64_t)rows};
+  cuuint64_t strides[2] = {128, (cuuint64_t)row_bytes};
+  cuuint32_t box[3] = {128, 1, (cuuint32_t)box_rows};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NQP, int NA>
+int launch_q8_tc(const Q8AttnParams& ap, const CUtensorMap& tk, const CUtensorMap& tv, const TailMaps& tails, int sms,
+                 cudaStream_t st) {
+  using C = Q8Cfg<NQP>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WFD_ERR_CUDA;
+  if (!attr_set[dev].load()) {
+    if (cudaFuncSetAttribute(q8_tc_kernel<NQP, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
+        cudaSuccess)
+      return WFD_ERR_CUDA;
+    attr_set[dev].store(true);
+  }
+  return launch_pdl(q8_tc_kernel<NQP, NA>, dim3(sms), dim3(q8_tc_threads(NA)), C::SMEM, st, tk, tv, tails, ap) ==
+                 cudaSuccess
+             ? WFD_OK
+             : WFD_ERR_CUDA;
+}
+
+template <typename T, int DH>
+int launch_q8_simt(int nq, const Q8AttnParams& ap, int sms, cudaStream_t st) {
+  const dim3 g(sms), b(kQ8SimtThreads);
+  cudaError_t e = nq == 1   ? launch_pdl(q8_attn_kernel<T, DH, 1>, g, b, 0, st, ap)
+                  : nq == 2 ? launch_pdl(q8_attn_kernel<T, DH, 2>, g, b, 0, st, ap)
+                            : launch_pdl(q8_attn_kernel<T, DH, 4>, g, b, 0, st, ap);
+  return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" size_t wfd_q8_cache_bytes(void) { return sizeof(wfd_q8_cache); }
+
+extern "C" int wfd_append_q8(const wfd_q8_cache* cache, const void* k_new, const void* v_new, const int32_t* slots,
+                             const int32_t* seqs, const int32_t* positions, int32_t n, int32_t slot_offset,
+                             int32_t dtype, int32_t* d_err, void* stream) {
+  Q8Cache c;
+  const int rc = q8_cache(cache, 0, &c);
+  if (rc != WFD_OK) return rc;
+  if (n < 0 || n > WFD_Q8_MAX_APPEND) return WFD_ERR_INVALID_ARG;
+  if (dtype != WFD_DTYPE_BF16 && dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
+  if (n == 0) return WFD_OK;
+  if (!k_new || !v_new || !slots || !seqs || !positions) return WFD_ERR_INVALID_ARG;
+  if (!aligned16(k_new) || !aligned16(v_new)) return WFD_ERR_ALIGNMENT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int work = 2 * c.Hkv * (c.Dh / 8);
+  const int threads = work >= 384 ? 384 : (work + 31) / 32 * 32;
+  cudaError_t e;
+  if (dtype == WFD_DTYPE_BF16)
+    e = launch_pdl(q8_append_kernel<__nv_bfloat16>, dim3(n), dim3(threads), 0, st,
+                   static_cast<const __nv_bfloat16*>(k_new), static_cast<const __nv_bfloat16*>(v_new), c, cache->lens,
+                   slots, seqs, positions, n, slot_offset, d_err);
+  else
+    e = launch_pdl(q8_append_kernel<float>, dim3(n), dim3(threads), 0, st, static_cast<const float*>(k_new),
+                   static_cast<const float*>(v_new), c, cache->lens, slots, seqs, positions, n, slot_offset, d_err);
+  return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
+}
+
+extern "C" int wfd_write_prefill_q8(const wfd_q8_cache* cache, const void* k, const void* v, int32_t slot, int32_t L,
+                                    int32_t dtype, int32_t* d_err, void* stream) {
+  Q8Cache c;
+  const int rc = q8_cache(cache, 0, &c);
+  if (rc != WFD_OK) return rc;
+  if (slot < 0 || slot >= c.n_slots || L < 0 || L > c.max_seq || c.n_seqs > 65535) return WFD_ERR_INVALID_ARG;
+  if (dtype != WFD_DTYPE_BF16 && dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
+  if (L == 0) return WFD_OK;
+  if (!k || !v) return WFD_ERR_INVALID_ARG;
+  if (!aligned16(k) || !aligned16(v)) return WFD_ERR_ALIGNMENT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid((L + kQ8Chunk - 1) / kQ8Chunk, c.n_seqs, 2);
+  const size_t smem = (size_t)c.Hkv * kQ8Chunk;
+  cudaError_t e;
+  if (dtype == WFD_DTYPE_BF16)
+    e = launch_pdl(q8_prefill_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), smem, st,
+                   static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), c, cache->lens, slot, L,
+                   d_err);
+  else
+    e = launch_pdl(q8_prefill_kernel<float>, grid, dim3(kQ8Threads), smem, st, static_cast<const float*>(k),
+                   static_cast<const float*>(v), c, cache->lens, slot, L, d_err);
+  return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
+}
+
+extern "C" int wfd_gather_q8(const wfd_q8_cache* cache, void* k_pack, void* v_pack, const int32_t* slots,
+                             const int32_t* seqs, const int32_t* cu_k, int32_t n, int64_t total, int32_t dtype,
+                             int32_t* d_err, void* stream) {
+  Q8Cache c;
+  const int rc = q8_cache(cache, 0, &c);
+  if (rc != WFD_OK) return rc;
+  if (n < 0 || n > 65535 || total < 0) return WFD_ERR_INVALID_ARG;
+  if (dtype != WFD_DTYPE_BF16 && dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
+  if (n == 0) return WFD_OK;
+  if (!slots || !seqs || !cu_k || (total > 0 && (!k_pack || !v_pack))) return WFD_ERR_INVALID_ARG;
+  if (!aligned16(k_pack) || !aligned16(v_pack)) return WFD_ERR_ALIGNMENT;
+  const int sms = current_sms();
+  if (sms <= 0) return WFD_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int chunks = (c.max_seq + kQ8Chunk - 1) / kQ8Chunk;
+  const int want = 32 * sms / (2 * n) + 1;  // lengths are device data: enough blocks to fill the GPU for any
+  const dim3 grid(chunks < want ? chunks : want, n, 2);
+  const size_t smem = (size_t)c.Hkv * kQ8Chunk;
+  cudaError_t e;
+  if (dtype == WFD_DTYPE_BF16)
+    e = launch_pdl(q8_gather_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), smem, st, c,
+                   static_cast<__nv_bfloat16*>(k_pack), static_cast<__nv_bfloat16*>(v_pack), slots, seqs, cu_k,
+                   (long long)total, d_err);
+  else
+    e = launch_pdl(q8_gather_kernel<float>, grid, dim3(kQ8Threads), smem, st, c, static_cast<float*>(k_pack),
+                   static_cast<float*>(v_pack), slots, seqs, cu_k, (long long)total, d_err);
+  return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
+}
+
+extern "C" int wfd_commit_window_q8(const wfd_q8_cache* cache, const wfd_item* items, int32_t n_items,
+                                    const int32_t* accept_len, const uint8_t* accept_mask, int32_t* acc_rows,
+                                    int32_t* acc_count, int32_t n_rows, int32_t slot_offset, int32_t* d_err,
+                                    void* stream) {
+  Q8Cache c;
+  const int rc = q8_cache(cache, 0, &c);
+  if (rc != WFD_OK) return rc;
+  if (n_items < 0 || n_rows < 0 || !cache->lens) return WFD_ERR_INVALID_ARG;
+  if ((accept_len == nullptr) == (accept_mask == nullptr)) return WFD_ERR_INVALID_ARG;
+  if (n_items == 0) return WFD_OK;
+  if (!items) return WFD_ERR_INVALID_ARG;
+  return launch_pdl(q8_commit_window_kernel, dim3(n_items), dim3(kCommitThreads), 0, static_cast<cudaStream_t>(stream),
+                    c, cache->lens, items, accept_len, accept_mask, acc_rows, acc_count, n_rows, slot_offset,
+                    d_err) == cudaSuccess
+             ? WFD_OK
+             : WFD_ERR_CUDA;
+}
+
+extern "C" size_t wfd_wave_attn_q8_workspace(int32_t n_items) {
+  const int sms = current_sms();
+  if (sms <= 0 || n_items < 0) return 0;
+  return ws_layout(n_items, 128, sms, true).total;
+}
+
+extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const void* q, const void* k_new,
+                                const void* v_new, void* out, const wfd_item* items, int32_t n_items, int32_t max_q,
+                                const int32_t* row_pos, int32_t row_pos_stride, int32_t slot_offset, int32_t n_rows,
+                                int32_t n_heads, int32_t dtype, float scale, void* workspace, size_t workspace_bytes,
+                                int32_t* d_err, void* stream) {
+  Q8Cache c;
+  const int rc = q8_cache(cache, slot_offset, &c);
+  if (rc != WFD_OK) return rc;
+  if (n_items < 0 || n_rows < 0 || n_heads <= 0 || n_heads % c.Hkv != 0 || max_q < 1 || which < -1 || which > 1)
+    return WFD_ERR_INVALID_ARG;
+  if (row_pos != nullptr && row_pos_stride < 1) return WFD_ERR_INVALID_ARG;
+  if (!(scale >= 0.f) || scale > 1e30f) return WFD_ERR_INVALID_ARG;
+  if (dtype != WFD_DTYPE_BF16 && dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
+  const int Dh = c.Dh, G = n_heads / c.Hkv;
+  if (Dh != 64 && Dh != 128) return WFD_ERR_UNSUPPORTED;
+  if (n_items == 0) return WFD_OK;
+  if (!q || !k_new || !v_new || !out || !items || !workspace) return WFD_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(out) || !aligned16(workspace))
+    return WFD_ERR_ALIGNMENT;
+  const int sms = current_sms();
+  if (sms <= 0) return WFD_ERR_CUDA;
+  // The tensor-core kernel reads rows of whole 128-byte heads (TMA) at int32 row
+  // coordinates; everything else runs on the CUDA cores.
+  const long long key_rows = (long long)cache->n_slots * c.n_seqs * c.max_seq;
+  const bool pair = Dh == 64;
+  const bool tc_ok = dtype == WFD_DTYPE_BF16 && (c.Hkv * Dh) % 128 == 0 && key_rows < (1ll << 31);
+  if (which < 0) which = tc_ok ? 1 : 0;
+  if (which == 1 && !tc_ok) return WFD_ERR_UNSUPPORTED;
+  const WsLayout L = ws_layout(n_items, 128, sms, true);
+  if (workspace_bytes < L.total) return WFD_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+
+  const bool tpair = which == 1 && pair;
+  const int Gv = tpair ? 2 * G : G;  // query vectors per window row and (pair of) kv head(s)
+  const long long nv = (long long)Gv * max_q;
+  const int NQ = which == 1 ? (nv <= 16 ? 16 : 32) : (nv == 1 ? 1 : nv == 2 ? 2 : kQ8SimtNQ);
+  static_assert(2 * kQ8SimtNQ * (128 + 2) <= 2 * kVerifyMaxRows * (128 + 2), "partials of the CUDA-core kernel");
+  const bool invariant = g_batch_invariant.load(std::memory_order_relaxed) != 0;
+  const bool self_plan = which == 1 && n_items <= kSelfPlanMax;
+  CUtensorMap tk, tv;
+  TailMaps tails;
+  if (which == 1) {
+    const int rb = c.Hkv * Dh;
+    if (!make_q8_map(&tk, cache->k, key_rows, rb, kTcTile) || !make_q8_map(&tv, cache->v, key_rows, rb, kTcTile))
+      return WFD_ERR_CUDA;
+    for (int pc = 0; pc < 4; ++pc)
+      if (!make_q8_map(&tails.k[pc], cache->k, key_rows, rb, 64 >> pc) ||
+          !make_q8_map(&tails.v[pc], cache->v, key_rows, rb, 64 >> pc))
+        return WFD_ERR_CUDA;
+  }
+
+  PlanParams pp;
+  memset(&pp, 0, sizeof(pp));
+  pp.mode = kPlanSlots;
+  pp.n = n_items;
+  pp.items = items;
+  pp.n_slots = c.n_slots;
+  pp.n_seqs = c.n_seqs;
+  pp.max_seq = c.max_seq;
+  pp.n_rows = n_rows;
+  pp.G = Gv;
+  pp.NQ = NQ;
+  pp.qg_split = 1;
+  pp.segs = reinterpret_cast<Seg*>(ws + L.segs);
+  pp.prefix = reinterpret_cast<long long*>(ws + L.prefix);
+  if (!self_plan) {
+    pp.start = reinterpret_cast<CtaStart*>(ws + L.start);
+    pp.seg_grid = sms;
+    pp.seg_units = tpair ? c.Hkv / 2 : c.Hkv;
+  }
+  pp.row_pos = row_pos;
+  pp.row_pos_stride = row_pos_stride;
+  pp.err = d_err;
+  pp.k_new = static_cast<const char*>(k_new);
+  pp.v_new = static_cast<const char*>(v_new);
+  pp.lens = cache->lens;
+  pp.lens_offset = slot_offset * c.n_seqs;
+  pp.q8 = c;
+  pp.zero = reinterpret_cast<int*>(ws + L.cnt);
+  pp.n_zero = sms;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 plan_grid(1 + (n_items < 4 * sms ? n_items : 4 * sms));
+  const cudaError_t pe = dtype == WFD_DTYPE_BF16
+                             ? launch_pdl(plan_kernel<__nv_bfloat16>, plan_grid, dim3(kPlanThreads), 0, st, pp)
+                             : launch_pdl(plan_kernel<float>, plan_grid, dim3(kPlanThreads), 0, st, pp);
+  if (pe != cudaSuccess) return WFD_ERR_CUDA;
+
+  Q8AttnParams ap;
+  memset(static_cast<void*>(&ap), 0, sizeof(ap));
+  ap.q = q;
+  ap.out = out;
+  ap.segs = pp.segs;
+  ap.prefix = pp.prefix;
+  ap.start = pp.start;
+  ap.n_segs = n_items;
+  ap.Hq = n_heads;
+  ap.Hkv = tpair ? c.Hkv / 2 : c.Hkv;
+  ap.G = G;
+  ap.pair = tpair ? 1 : 0;
+  ap.invariant = invariant ? 1 : 0;
+  ap.scale_log2 = (scale > 0.f ? scale : 1.0f / std::sqrt((float)Dh)) * 1.4426950408889634f;
+  ap.causal = 1;
+  ap.k_row_offset = (long long)slot_offset * c.n_seqs * c.max_seq;
+  ap.ws_part = reinterpret_cast<float*>(ws + L.part);
+  ap.ws_cnt = pp.zero;
+  ap.err = d_err;
+  ap.fail_waits = g_fail_waits.load(std::memory_order_relaxed);
+  ap.row_pos = row_pos;
+  ap.row_pos_stride = row_pos_stride;
+  ap.c = c;
+  if (which == 0) {
+    if (dtype == WFD_DTYPE_BF16)
+      return Dh == 128 ? launch_q8_simt<__nv_bfloat16, 128>(NQ, ap, sms, st)
+                       : launch_q8_simt<__nv_bfloat16, 64>(NQ, ap, sms, st);
+    return Dh == 128 ? launch_q8_simt<float, 128>(NQ, ap, sms, st) : launch_q8_simt<float, 64>(NQ, ap, sms, st);
+  }
+  if (self_plan) {
+    ap.items = items;
+    ap.n_slots = c.n_slots;
+    ap.n_seqs = c.n_seqs;
+    ap.max_seq = c.max_seq;
+    ap.n_rows = n_rows;
+    ap.Gv = Gv;
+    ap.NQ = NQ;
+  }
+  if (NQ == 32) return launch_q8_tc<32, 32>(ap, tk, tv, tails, sms, st);
+  if (nv <= 2) return launch_q8_tc<16, 2>(ap, tk, tv, tails, sms, st);
+  if (nv <= 4) return launch_q8_tc<16, 4>(ap, tk, tv, tails, sms, st);
+  if (nv <= 8) return launch_q8_tc<16, 8>(ap, tk, tv, tails, sms, st);
+  return launch_q8_tc<16, 16>(ap, tk, tv, tails, sms, st);
+}

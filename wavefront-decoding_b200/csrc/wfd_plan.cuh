@@ -9,7 +9,10 @@
 // graph_blocks.py:5-11).
 #pragma once
 
+#include <type_traits>
+
 #include "wfd_common.cuh"
+#include "wfd_q8.cuh"
 
 namespace wfd {
 
@@ -60,6 +63,11 @@ struct PlanParams {
   // an item sits at row_pos[(q_row0 + j) * row_pos_stride]
   const int32_t* row_pos;
   int row_pos_stride;
+  // window append into an 8-bit cache (plan_kernel<T>: k_new / v_new hold T rows);
+  // its slots and the items' are both counted from the call's slot offset
+  Q8Cache q8;
+  int* zero;  // plan_kernel<T>: arrival counters cleared for the attention (n_zero)
+  int n_zero;
 };
 
 constexpr int kPlanThreads = 1024;
@@ -95,9 +103,77 @@ __device__ __forceinline__ long long block_excl_scan(long long x, long long* war
   return r;
 }
 
+// Window append into an 8-bit cache (blocks 1.. of the plan kernel): the rows are
+// quantised on the way.  Where two items of a call hold the same position of one
+// (slot, sequence) the later item's row is stored, codes and exponent of one row.
+template <typename T>
+__device__ __forceinline__ void plan_append_q8(const PlanParams& p) {
+  for (int i = blockIdx.x - 1; i < p.n; i += gridDim.x - 1) {
+    const wfd_item it = p.items[i];
+    int last = 0;
+    if (it.q_len <= 0 ||
+        check_slot_item(it, p.n_slots, p.n_seqs, p.max_seq, p.n_rows, p.row_pos, p.row_pos_stride, last) != 0)
+      continue;
+    auto at = [&](const wfd_item& x, int j) {
+      return p.row_pos != nullptr ? p.row_pos[((long long)x.q_row0 + j) * p.row_pos_stride] : x.pos0 + j;
+    };
+    // position of row j, or -1: a gapped window's row out of order is skipped and reported
+    auto pos_of = [&](int j) {
+      const int pos = at(it, j);
+      if (p.row_pos != nullptr && (pos < it.pos0 || pos > last || (j + 1 < it.q_len && at(it, j + 1) <= pos))) {
+        set_error(p.err, kErrBadPos);
+        return -1;
+      }
+      return pos;
+    };
+    // a later valid item on the same (slot, sequence), or one that holds position pos there
+    auto later = [&](int pos) {
+      int found = 0;
+      for (int k = i + 1 + threadIdx.x; k < p.n && !found; k += blockDim.x) {
+        const wfd_item o = p.items[k];
+        int ol = 0;
+        if (o.slot != it.slot || o.seq != it.seq || o.q_len <= 0 ||
+            check_slot_item(o, p.n_slots, p.n_seqs, p.max_seq, p.n_rows, p.row_pos, p.row_pos_stride, ol) != 0)
+          continue;
+        if (pos < 0) {
+          found = 1;
+        } else if (p.row_pos == nullptr) {
+          found = pos >= o.pos0 && pos <= ol;
+        } else {
+          for (int j = 0; j < o.q_len; ++j) found |= at(o, j) == pos;
+        }
+      }
+      return __syncthreads_or(found);
+    };
+    const T* kn = reinterpret_cast<const T*>(p.k_new);
+    const T* vn = reinterpret_cast<const T*>(p.v_new);
+    if (!later(-1)) {
+      q8_put_rows(kn, vn, it.q_row0, it.q_len, p.q8, it.slot, it.seq, pos_of, p.err);
+    } else {
+      for (int j = 0; j < it.q_len; ++j) {
+        const int pos = pos_of(j);
+        if (pos < 0 || later(pos)) continue;
+        q8_put_rows(kn, vn, (long long)it.q_row0 + j, 1, p.q8, it.slot, it.seq, [&](int) { return pos; }, p.err);
+      }
+    }
+    if (threadIdx.x == 0 && p.lens != nullptr)
+      atomicMax(p.lens + it.slot * p.n_seqs + it.seq + p.lens_offset, last + 1);
+  }
+}
+
+// TQ: void for caches of the rows' own type (the window append copies bytes), the
+// rows' type for an 8-bit cache.
+template <typename TQ>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   griddep_wait();  // launched with programmatic stream serialization (items come from the predecessor)
   griddep_launch_dependents();  // the attention kernel may run its prologue meanwhile
+  if constexpr (!std::is_void<TQ>::value) {
+    if (blockIdx.x > 0) {
+      plan_append_q8<TQ>(p);
+      return;
+    }
+    for (int i = threadIdx.x; i < p.n_zero; i += blockDim.x) p.zero[i] = 0;
+  }
   if (blockIdx.x > 0) {
     // ---- window append: the tensor-core kernel reads every key through TMA, so
     // the window rows go to the cache before it starts (it waits for this grid).

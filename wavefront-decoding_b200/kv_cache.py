@@ -10,9 +10,12 @@ of a host list, so appends, rollbacks and commits can run inside CUDA graphs.
 `seqlen` gives the reference's host view (it synchronises).  Every mutation is
 a libwfd_b200 kernel: append (write_tokens), prefill write, rollback
 (drop_positions_at_and_after) and the window accept/compact commit.
+
+`QuantKVCache` holds the same slots in 8 bits per element.
 """
 from __future__ import annotations
 
+import ctypes
 
 import torch
 
@@ -164,8 +167,164 @@ class SlotKVCache:
 
     # ------------------------------------------------------------------
     def wave_attn(self, q, k_new, v_new, items, max_q: int, *, slot_offset: int = 0, out=None, kernel: int = -1,
-                  update_lens: bool = True):
+                  update_lens: bool = True, row_pos=None):
         """Fused append + wavefront attention over this cache's slots."""
         return _attn.wave_attn(q, k_new, v_new, self.K, self.V, items, max_q,
                                lens=self.lens if update_lens else None, slot_offset=slot_offset, out=out,
-                               kernel=kernel)
+                               kernel=kernel, row_pos=row_pos)
+
+
+class QuantKVCache(SlotKVCache):
+    """A slot cache of 8-bit rows, quantised as they are written.
+
+    K, V: float8_e4m3fn codes in SlotKVCache's layout; k_exp, v_exp: int8 exponents
+    (n_slots, B, Hkv, max_seq_len), one per row of head_dim values.  A cached value
+    is code * 2^exp, exp the smallest integer with max|row| <= 448 * 2^exp (clamped
+    to [-32, 32]): the scale is a power of two, so the rounding to e4m3 (4
+    significant bits) is the only one.  Per element 1 + 1/Dh bytes instead of 2 or 4.
+
+    `dtype` is the type of the rows written and read back (bf16 or fp32); head_dim a
+    power of two from 16 to 256 (64 or 128 for wave_attn).  A NaN is stored as 0 and
+    reported through the device error word; an infinity saturates.  Rows given to
+    the methods may have any strides.  Same methods as SlotKVCache, whose lengths
+    and rollbacks it shares."""
+
+    def __init__(self, n_slots: int, batch_size: int, n_kv_head: int, head_dim: int, max_seq_len: int,
+                 dtype: torch.dtype, device: torch.device):
+        dev = torch.device(device)
+        shape = (n_slots, batch_size, max_seq_len, n_kv_head, head_dim)
+        eshape = (n_slots, batch_size, n_kv_head, max_seq_len)
+        self._adopt(torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                    torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                    torch.zeros(eshape, dtype=torch.int8, device=dev),
+                    torch.zeros(eshape, dtype=torch.int8, device=dev), None, dtype)
+
+    @classmethod
+    def wrap(cls, K: torch.Tensor, V: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+             lens: torch.Tensor | None = None, *, dtype: torch.dtype = torch.bfloat16) -> "QuantKVCache":
+        """Adopt existing code and exponent tensors without copying (every code finite)."""
+        self = cls.__new__(cls)
+        self._adopt(K, V, k_exp, v_exp, lens, dtype)
+        return self
+
+    def _adopt(self, K, V, k_exp, v_exp, lens, dtype) -> None:
+        rt.dtype_code(dtype)
+        if lens is None:
+            lens = torch.zeros(K.shape[:2], dtype=torch.int32, device=K.device)
+        self._c = _ops.q8_cache_struct(K, V, k_exp, v_exp, lens)
+        Dh = K.shape[4]
+        if Dh < 16 or Dh > 256 or Dh & (Dh - 1):
+            raise ValueError(f"head_dim {Dh}: an 8-bit cache takes powers of two from 16 to 256")
+        self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim = K.shape
+        self.dtype, self.device = dtype, K.device
+        self.K, self.V, self.k_exp, self.v_exp, self.lens = K, V, k_exp, v_exp, lens
+
+    @property
+    def nbytes(self) -> int:
+        return self.K.numel() + self.V.numel() + self.k_exp.numel() + self.v_exp.numel()
+
+    def _call(self, name: str, *args) -> None:
+        rt.call(self.device, name, ctypes.byref(self._c), *args, rt.error_word(self.device).data_ptr(),
+                self._stream())
+
+    def _rows(self, k, v, lead: tuple):
+        shape = (*lead, self.n_kv_head, self.head_dim)
+        if k.shape != shape or v.shape != shape:
+            raise ValueError(f"k, v must be {shape}, got {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype != v.dtype:
+            raise TypeError("k, v must share a dtype")
+        if rt.require_cuda(k, v) != self.device:
+            raise ValueError(f"rows on {k.device}, cache on {self.device}")
+        return rt.rows16(k), rt.rows16(v), rt.dtype_code(k.dtype)
+
+    def write_prefill(self, slot: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """k, v: (B, L, Hkv, Dh) prompt K/V, quantised to positions [0, L)."""
+        L = k.shape[1]
+        assert L <= self.S
+        k, v, dt = self._rows(k, v, (self.B, L))
+        self._call("wfd_write_prefill_q8", k.data_ptr(), v.data_ptr(), int(slot), L, dt)
+
+    def write_tokens(self, slots, seq_ids, positions, k: torch.Tensor, v: torch.Tensor, *, slot_offset: int = 0) -> None:
+        """Quantise n rows k, v (n, Hkv, Dh) to (slots[i], seq_ids[i], positions[i]);
+        where two rows name one place the later one is stored.  Bounds as
+        SlotKVCache.write_tokens."""
+        n = k.shape[0]
+        if isinstance(positions, list):
+            for p in positions:
+                if p >= self.S:
+                    raise IndexError(f"position {p} exceeds max_seq_len={self.S}")
+        sl, sq, ps = (_ops.i32(t, self.device) for t in (slots, seq_ids, positions))
+        if not sl.numel() == sq.numel() == ps.numel() == n:
+            raise ValueError(f"{n} rows need {n} slots, seq_ids and positions")
+        k, v, dt = self._rows(k, v, (n,))
+        step = _abi.WFD_Q8_MAX_APPEND
+        for i in range(0, n, step):
+            m = min(step, n - i)
+            self._call("wfd_append_q8", k[i:].data_ptr(), v[i:].data_ptr(), sl[i:].data_ptr(), sq[i:].data_ptr(),
+                       ps[i:].data_ptr(), m, int(slot_offset), dt)
+
+    def gather_packed(self, slots: torch.Tensor, seq_ids: torch.Tensor, cu_k: torch.Tensor, total: int, *, out=None):
+        """Read back: segment i holds the values of positions [0, cu_k[i+1] -
+        cu_k[i]) of (slots[i], seq_ids[i]) at rows cu_k[i].. of the (total, Hkv, Dh)
+        packs returned.  Device int32 tensors, whose contents may change between
+        CUDA-graph replays; segments that do not fit are skipped and reported.
+        `out`: (k_pack, v_pack) to write into."""
+        sl, sq, cu = (_ops.i32(t, self.device) for t in (slots, seq_ids, cu_k))
+        n = sl.numel()
+        if sq.numel() != n or cu.numel() != n + 1:
+            raise ValueError("gather_packed: n slots and seq_ids need n + 1 entries of cu_k")
+        shape = (int(total), self.n_kv_head, self.head_dim)
+        if out is None:
+            out = tuple(torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
+        k_pack, v_pack = out
+        for t in out:
+            if tuple(t.shape) != shape or t.dtype != self.dtype or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"gather_packed: packs must be contiguous {self.dtype} {shape} on {self.device}")
+        self._call("wfd_gather_q8", k_pack.data_ptr(), v_pack.data_ptr(), sl.data_ptr(), sq.data_ptr(), cu.data_ptr(),
+                   n, int(total), rt.dtype_code(self.dtype))
+        return k_pack, v_pack
+
+    def gather_pack(self, slots, seq_ids, uptos):
+        """SlotKVCache.gather_pack with the values dequantised to `dtype`."""
+        lengths = [u + 1 for u in uptos]
+        cu = [0]
+        for ln in lengths:
+            cu.append(cu[-1] + ln)
+        cu_k = torch.tensor(cu, dtype=torch.int32, device=self.device)
+        k_pack, v_pack = self.gather_packed(slots, seq_ids, cu_k, cu[-1])
+        return k_pack, v_pack, cu_k, max(lengths)
+
+    def commit_window(self, items: torch.Tensor, *, accept_len: torch.Tensor | None = None,
+                      accept_mask: torch.Tensor | None = None, slot_offset: int = 0, n_rows: int | None = None,
+                      out: tuple[torch.Tensor, torch.Tensor] | None = None):
+        """SlotKVCache.commit_window: accepted rows move as they are, codes and exponents."""
+        if (accept_len is None) == (accept_mask is None):
+            raise ValueError("give exactly one of accept_len / accept_mask")
+        items = _ops.i32(items, self.device).reshape(-1, 5)
+        n = items.shape[0]
+        al = None if accept_len is None else _ops.i32(accept_len, self.device)
+        am = None
+        if accept_mask is not None:
+            am = torch.as_tensor(accept_mask).to(device=self.device, dtype=torch.uint8).contiguous()
+        if out is None:
+            if n_rows is None:
+                n_rows = int((items[:, 4] + items[:, 3]).max().item()) if n else 0
+            out = (torch.full((int(n_rows),), -1, dtype=torch.int32, device=self.device),
+                   torch.zeros(n, dtype=torch.int32, device=self.device))
+        acc_rows, acc_count = out
+        for t in out:
+            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+                raise ValueError("acc_rows / acc_count must be contiguous int32 tensors on the cache's device")
+        if acc_count.numel() < n or (al is not None and al.numel() < n):
+            raise ValueError("acc_count and accept_len need one entry per item")
+        rows = acc_rows.numel() if am is None else min(acc_rows.numel(), am.numel())
+        self._call("wfd_commit_window_q8", items.data_ptr(), n, rt.ptr(al), rt.ptr(am), acc_rows.data_ptr(),
+                   acc_count.data_ptr(), rows, int(slot_offset))
+        return (acc_rows if n_rows is None else acc_rows[:n_rows]), acc_count[:n]
+
+    def wave_attn(self, q, k_new, v_new, items, max_q: int, *, slot_offset: int = 0, out=None, kernel: int = -1,
+                  update_lens: bool = True, row_pos=None):
+        """Fused quantising append + wavefront attention over this cache's slots."""
+        return _attn.wave_attn_q8(q, k_new, v_new, self.K, self.V, self.k_exp, self.v_exp, items, max_q,
+                                  lens=self.lens if update_lens else None, slot_offset=slot_offset, out=out,
+                                  kernel=kernel, row_pos=row_pos)

@@ -29,8 +29,16 @@ dispatcher.
   wfd::commit_out(..., Tensor(d!) acc_rows, Tensor(e!) acc_count) -> ()
   wfd::commit_drop(lens!, drop_pos) -> ()
       batched drop_positions_at_and_after (drop_pos[b] = -1 keeps sequence b).
+  wfd::wave_attn_q8(q, k_new, v_new, k_cache!, v_cache!, k_exp!, v_exp!, items,
+                    max_q, lens!?=None, slot_offset=0, scale=None, kernel=-1,
+                    row_pos=None) -> out
+      wave_attn over an 8-bit cache (kv_cache.QuantKVCache): the window rows are
+      quantised into it, and every key is attended as the cache holds it.
+  wfd::wave_attn_q8_out(..., Tensor(f!) out) -> ()
 """
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -56,6 +64,13 @@ _SCHEMAS = {
                   "Tensor? accept_len, Tensor? accept_mask, int slot_offset, Tensor(d!) acc_rows, "
                   "Tensor(e!) acc_count) -> ()",
     "commit_drop": "commit_drop(Tensor(a!) lens, Tensor drop_pos) -> ()",
+    "wave_attn_q8": "wave_attn_q8(Tensor q, Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+                    "Tensor(c!) k_exp, Tensor(d!) v_exp, Tensor items, int max_q, Tensor(e!)? lens=None, "
+                    "int slot_offset=0, float? scale=None, int kernel=-1, Tensor? row_pos=None) -> Tensor",
+    "wave_attn_q8_out": "wave_attn_q8_out(Tensor q, Tensor k_new, Tensor v_new, Tensor(a!) k_cache, "
+                        "Tensor(b!) v_cache, Tensor(c!) k_exp, Tensor(d!) v_exp, Tensor items, int max_q, "
+                        "Tensor(e!)? lens, int slot_offset, float? scale, int kernel, Tensor? row_pos, "
+                        "Tensor(f!) out) -> ()",
 }
 for _schema in _SCHEMAS.values():
     _LIB.define(_schema)
@@ -124,6 +139,25 @@ def _check_commit(k_cache, v_cache, lens, items, accept_len, accept_mask):
     if accept_mask is not None and accept_mask.dtype != torch.uint8:
         raise ValueError("accept_mask must be uint8")
     return dev
+
+
+def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
+    """The C view of an 8-bit cache's tensors, after the checks of their shapes and types."""
+    if k.dim() != 5 or v.shape != k.shape or k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or \
+            not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("K, V must be contiguous float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) tensors")
+    n_slots, n_seqs, max_seq, Hkv, Dh = k.shape
+    want = (n_slots, n_seqs, Hkv, max_seq)
+    for e in (k_exp, v_exp):
+        if e.dtype != torch.int8 or tuple(e.shape) != want or not e.is_contiguous():
+            raise ValueError("k_exp, v_exp must be contiguous int8 (n_slots, n_seqs, Hkv, max_seq) tensors")
+    if lens is not None and (lens.dtype != torch.int32 or tuple(lens.shape) != (n_slots, n_seqs) or
+                             not lens.is_contiguous()):
+        raise ValueError("lens must be a contiguous int32 (n_slots, n_seqs) tensor")
+    c = _abi.wfd_q8_cache()
+    c.k, c.v, c.k_exp, c.v_exp, c.lens = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), rt.ptr(lens)
+    c.n_slots, c.n_seqs, c.max_seq, c.n_kv_heads, c.head_dim = n_slots, n_seqs, max_seq, Hkv, Dh
+    return c
 
 
 # ---------------------------------------------------------------------------
@@ -220,6 +254,55 @@ def _commit_drop_cuda(lens, drop_pos):
     _abi.check(st, "wfd_commit_drop")
 
 
+def _wave_attn_q8_out_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens, slot_offset, scale,
+                           kernel, row_pos, out):
+    dev = rt.require_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, lens, row_pos, out)
+    c = q8_cache_struct(k_cache, v_cache, k_exp, v_exp, lens)
+    Hkv, Dh = k_cache.shape[3:]
+    if q.dim() != 3 or q.shape[2] != Dh or k_new.shape != (q.shape[0], Hkv, Dh) or v_new.shape != k_new.shape:
+        raise ValueError("q (n_rows, H, Dh) and k_new / v_new (n_rows, Hkv, Dh) must match the cache")
+    if q.dtype != k_new.dtype or q.dtype != v_new.dtype:
+        raise TypeError("q, k_new, v_new must share a dtype")
+    if q.shape[1] % Hkv != 0:
+        raise ValueError(f"query heads {q.shape[1]} not a multiple of kv heads {Hkv}")
+    if items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 5 or not items.is_contiguous():
+        raise ValueError("items must be a contiguous int32 (n_items, 5) device tensor")
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor shaped like q")
+    rp_stride = 1
+    if row_pos is not None:
+        if row_pos.dtype != torch.int32 or row_pos.dim() != 1 or row_pos.numel() < q.shape[0] or \
+                (row_pos.numel() > 1 and row_pos.stride(0) < 1):
+            raise ValueError("row_pos must be an int32 device vector with one position per q row")
+        rp_stride = max(1, row_pos.stride(0))
+    q, k_new, v_new = rt.rows16(q), rt.rows16(k_new), rt.rows16(v_new)
+    n = items.shape[0]
+    # scratch of this call alone: calls on several streams, and graphs replayed side
+    # by side, share nothing
+    wsb = q8_workspace_bytes(dev, n)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    rt.call(dev, "wfd_wave_attn_q8", int(kernel), ctypes.byref(c), q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+            out.data_ptr(), items.data_ptr(), n, int(max_q), rt.ptr(row_pos), rp_stride, int(slot_offset), q.shape[0],
+            q.shape[1], rt.dtype_code(q.dtype), float(scale or 0.0), ws.data_ptr(), wsb,
+            rt.error_word(dev).data_ptr(), rt.stream_ptr(dev))
+
+
+def q8_workspace_bytes(dev: torch.device, n: int) -> int:
+    with torch.cuda.device(dev):
+        b = int(_abi.load().wfd_wave_attn_q8_workspace(n))
+    if b <= 0:
+        raise _abi.WfdError("wfd_wave_attn_q8_workspace", -1, "could not size the workspace")
+    return b
+
+
+def _wave_attn_q8_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens=None, slot_offset=0,
+                       scale=None, kernel=-1, row_pos=None):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _wave_attn_q8_out_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens, slot_offset, scale,
+                           kernel, row_pos, out)
+    return out
+
+
 _LIB.impl("attn", _attn_cuda, "CUDA")
 _LIB.impl("attn_out", _attn_out_cuda, "CUDA")
 _LIB.impl("wave_attn", _wave_attn_cuda, "CUDA")
@@ -227,6 +310,8 @@ _LIB.impl("wave_attn_out", _wave_attn_out_cuda, "CUDA")
 _LIB.impl("commit", _commit_cuda, "CUDA")
 _LIB.impl("commit_out", _commit_out_cuda, "CUDA")
 _LIB.impl("commit_drop", _commit_drop_cuda, "CUDA")
+_LIB.impl("wave_attn_q8", _wave_attn_q8_cuda, "CUDA")
+_LIB.impl("wave_attn_q8_out", _wave_attn_q8_out_cuda, "CUDA")
 
 
 # ---------------------------------------------------------------------------
@@ -266,4 +351,16 @@ def _commit_out_fake(k_cache, v_cache, lens, items, accept_len, accept_mask, slo
 
 @torch.library.register_fake("wfd::commit_drop")
 def _commit_drop_fake(lens, drop_pos):
+    return None
+
+
+@torch.library.register_fake("wfd::wave_attn_q8")
+def _wave_attn_q8_fake(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens=None, slot_offset=0,
+                       scale=None, kernel=-1, row_pos=None):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+@torch.library.register_fake("wfd::wave_attn_q8_out")
+def _wave_attn_q8_out_fake(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens, slot_offset, scale,
+                           kernel, row_pos, out):
     return None

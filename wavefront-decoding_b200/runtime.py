@@ -54,6 +54,24 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous at a 16-byte aligned address (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def call(device: torch.device, name: str, *args) -> None:
+    """Run entry point `name` with `device` current (its launches go to the
+    current device, whatever device the stream belongs to) and check its status."""
+    fn = getattr(_abi.load(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        st = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args)
+    _abi.check(st, name)
+
+
 def _capturing() -> bool:
     return torch.cuda.is_current_stream_capturing()
 
