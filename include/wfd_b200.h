@@ -437,6 +437,47 @@ int wfd_items_from_table(const int32_t* tab, int32_t cols, int32_t c_slot, int32
 /* Greedy ids: out[r] = the first index of the maximum of logits row r (n rows of V). */
 int wfd_argmax_rows(const void* x, int32_t* out, int32_t n, int32_t V, int32_t dtype, void* stream);
 
+/* Sampled ids: out[r] is drawn from logits row r by the uniform number u (no
+ * counterpart in the reference, which decodes greedily).  With m0 = max x, T the
+ * temperature and w_i = exp((x_i - m0) / T), in the order "x descending, index
+ * ascending":
+ *   top_k  keeps the first top_k tokens         (top_k <= 0 or >= V: all)
+ *   top_p  of these, every token whose predecessors weigh less than top_p times
+ *          all of them; the first in any case     (top_p >= 1: all)
+ *   min_p  of these, w_i >= min_p                (min_p <= 0: all; > 1 counts as 1)
+ * and out[r] is the first index, in index order, at which the kept weight up to
+ * and including it exceeds u times the kept weight (u < 0 or NaN counts as 0; u >= 1
+ * gives the last kept token).  T <= 0 or NaN: the first index of the maximum.  A NaN
+ * logit counts as -inf; +inf logits share the row equally; a row of -inf gives -1.
+ * Weights and sums are held in 64 bits, exact in any order: the id depends on the
+ * row, its parameters and u only.  Weights below 2^-45 of the largest count as 0.
+ * V <= 2^19.
+ *
+ * Row r takes its parameters at index row_seq[r * seq_stride] (r when row_seq is
+ * NULL) of the four parameter vectors (each n_params long; NULL: temperature 1, no
+ * filter) and u at u[index * u_stride + row_pos[r * pos_stride]] (column 0 when
+ * row_pos is NULL): a tick table's sequence and position columns select each
+ * row's request and the number reserved for that position.  An index outside
+ * [0, n_params) or [0, u_cols) gives -1 and is reported (error bit 8). */
+typedef struct wfd_sample_params {
+  const void* x;             /* (n, V) logits, row stride ldx elements */
+  int32_t* out;              /* (n)                                     */
+  const float* u;            /* (n_params, u_cols), row stride u_stride */
+  const float* temperature;  /* (n_params) or NULL, and the next three   */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const int32_t* row_seq;    /* or NULL */
+  const int32_t* row_pos;    /* or NULL */
+  int32_t* err;
+  int64_t ldx;
+  int32_t n, V, dtype, n_params, u_stride, u_cols, seq_stride, pos_stride;
+} wfd_sample_params;
+
+int wfd_sample_rows(const wfd_sample_params* p, void* stream);
+/* sizeof(wfd_sample_params) as compiled into the library. */
+size_t wfd_sample_params_bytes(void);
+
 /* ---------------------------------------------------------------------------
  * Device-side wavefront scheduling (route / settle of scheduler_batch.py:268-360
  * as kernels, so one CUDA graph runs a whole tick; no counterpart in the

@@ -31,6 +31,7 @@ EXPORTED = (
     "wfd_linear", "wfd_linear_params_bytes", "wfd_rope_split_norm", "wfd_silu_mul_norm",
     "wfd_q8_cache_bytes", "wfd_append_q8", "wfd_write_prefill_q8", "wfd_gather_q8", "wfd_commit_window_q8",
     "wfd_wave_attn_q8", "wfd_wave_attn_q8_workspace",
+    "wfd_sample_rows", "wfd_sample_params_bytes",
 )
 WFD_Q8_MAX_APPEND = 16384
 
@@ -77,6 +78,15 @@ class wfd_q8_cache(ctypes.Structure):
     """include/wfd_b200.h: wfd_q8_cache (field order and types must match)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_exp", "v_exp", "lens")] + \
         [(n, ctypes.c_int32) for n in ("n_slots", "n_seqs", "max_seq", "n_kv_heads", "head_dim")]
+
+
+class wfd_sample_params(ctypes.Structure):
+    """include/wfd_b200.h: wfd_sample_params (field order and types must match)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "x", "out", "u", "temperature", "top_k", "top_p", "min_p", "row_seq", "row_pos", "err")] + \
+        [("ldx", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("n", "V", "dtype", "n_params", "u_stride", "u_cols", "seq_stride",
+                                       "pos_stride")]
 
 
 _P = ctypes.c_void_p
@@ -155,6 +165,9 @@ _SIGS = {
     "wfd_wave_attn_q8_workspace": ([_I], _S),
     # which cache q k_new v_new out items n max_q row_pos rp_stride slot_off n_rows Hq dtype scale ws ws_bytes err stream
     "wfd_wave_attn_q8": ([_I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _F, _P, _S, _P, _P], _I),
+    # const wfd_sample_params*, stream
+    "wfd_sample_rows": ([_P, _P], _I),
+    "wfd_sample_params_bytes": ([], _S),
     # const wfd_sched_params*, stream
     "wfd_sched_pre_tick": ([_P, _P], _I),
     "wfd_sched_route": ([_P, _P], _I),

@@ -17,6 +17,7 @@
 #include "wfd_decode.cuh"
 #include "wfd_linear.cuh"
 #include "wfd_model.cuh"
+#include "wfd_sample.cuh"
 #include "wfd_sched.cuh"
 #include "wfd_plan.cuh"
 #include "wfd_prefill.cuh"
@@ -1632,4 +1633,83 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   if (nv <= 4) return launch_q8_tc<16, 4>(ap, tk, tv, tails, sms, st);
   if (nv <= 8) return launch_q8_tc<16, 8>(ap, tk, tv, tails, sms, st);
   return launch_q8_tc<16, 16>(ap, tk, tv, tails, sms, st);
+}
+
+// ---------------------------------------------------------------------------
+// sampling
+// ---------------------------------------------------------------------------
+namespace {
+template <typename T>
+int launch_sample(const SampleParams& p, int cluster, size_t smem, cudaStream_t st) {
+  static std::atomic<bool> attr_set[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WFD_ERR_CUDA;
+  if (!attr_set[dev].load()) {
+    constexpr int most = (int)sizeof(SampleShared) + kSampleMaxV / 256 * 8;
+    if (cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+      return WFD_ERR_CUDA;
+    attr_set[dev].store(true);
+  }
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)p.n * cluster);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, p) == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
+}
+}  // namespace
+
+extern "C" size_t wfd_sample_params_bytes(void) { return sizeof(wfd_sample_params); }
+
+extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
+  if (!a || a->n < 0 || a->V <= 0 || a->V > kSampleMaxV || a->ldx < a->V) return WFD_ERR_INVALID_ARG;
+  if (a->dtype != WFD_DTYPE_BF16 && a->dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
+  if (a->n == 0) return WFD_OK;
+  if (!a->x || !a->out || !a->u || !a->err) return WFD_ERR_INVALID_ARG;
+  if (a->n_params <= 0 || a->u_cols <= 0 || a->u_stride < a->u_cols) return WFD_ERR_INVALID_ARG;
+  if (!a->row_seq && a->n_params < a->n) return WFD_ERR_INVALID_ARG;
+  if ((a->row_seq && a->seq_stride < 1) || (a->row_pos && a->pos_stride < 1)) return WFD_ERR_INVALID_ARG;
+  const int eb = elem_bytes(a->dtype);
+  if (reinterpret_cast<uintptr_t>(a->x) % eb != 0) return WFD_ERR_ALIGNMENT;
+  const int sms = current_sms();
+  if (sms <= 0) return WFD_ERR_CUDA;
+  SampleParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x;
+  p.out = a->out;
+  p.u = a->u;
+  p.temperature = a->temperature;
+  p.top_k = a->top_k;
+  p.top_p = a->top_p;
+  p.min_p = a->min_p;
+  p.row_seq = a->row_seq;
+  p.row_pos = a->row_pos;
+  p.err = a->err;
+  p.ldx = a->ldx;
+  p.n = a->n;
+  p.V = a->V;
+  p.vec = aligned16(a->x) && (a->ldx * eb) % 16 == 0 ? 1 : 0;
+  p.n_params = a->n_params;
+  p.u_stride = a->u_stride;
+  p.u_cols = a->u_cols;
+  p.seq_stride = a->seq_stride;
+  p.pos_stride = a->pos_stride;
+  // CTAs per row: as many as fit at two CTAs an SM, with at least a tile of tokens each
+  int cluster = 1;
+  while (cluster < 8 && (long long)a->n * cluster * 2 <= 2ll * sms && cluster * kSampleTile < a->V) cluster *= 2;
+  p.slice = ((a->V + cluster - 1) / cluster + kSampleTile - 1) / kSampleTile * kSampleTile;
+  const size_t smem = sizeof(SampleShared) + (size_t)p.slice / 256 * 8;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->dtype == WFD_DTYPE_BF16 ? launch_sample<__nv_bfloat16>(p, cluster, smem, st)
+                                    : launch_sample<float>(p, cluster, smem, st);
 }

@@ -3,11 +3,14 @@
 rmsnorm     one launch per call instead of up-cast / pow / mean / rsqrt / mul / down-cast
 rope_split  fused-QKV output -> contiguous q, k (RoPE at per-row positions) and v
 silu_mul    SwiGLU gate silu(g) * u
+sample_rows ids drawn with temperature, top-k, top-p and min-p from given uniform numbers
 gather_rows / scatter_rows / items_from_table / argmax_rows: state-pool row
             plumbing and greedy ids by int32 indices (no int64 index tensors)
 All arithmetic is fp32; storage bf16 or fp32.  No CPU path: CPU tensors raise.
 """
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -154,6 +157,63 @@ def argmax_rows(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def sample_rows(x: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | None = None,
+                top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                min_p: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
+                row_pos: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sampled ids (int32, one per row) of logits x (n, V), bf16 or fp32 (padded rows,
+    x.stride(0) > V, are read in place).
+
+    With w_i = exp((x_i - max x) / temperature), in the order "x descending, index
+    ascending": top_k keeps the first tokens (<= 0: all), top_p of these the ones
+    whose predecessors weigh less than top_p of them (>= 1: all; the first always),
+    min_p of these the ones with w_i >= min_p (<= 0: all); the id is the first index,
+    in index order, at which the kept weight so far exceeds u times all of it.
+    temperature <= 0 is greedy (argmax_rows).  NaN logits count as -inf; a row of
+    -inf gives -1.  Sums are exact, so an id depends on its row, parameters and u only.
+
+    temperature, top_p, min_p: fp32, top_k: int32, one entry per row, or None (1, no
+    filter).  u: fp32 numbers in [0, 1), one per row.  With row_seq (int32, any
+    stride) row r takes entry row_seq[r] of these vectors instead, and with row_pos
+    u is (entries, columns) and row r takes u[entry, row_pos[r]]."""
+    dev = rt.require_cuda(x, u, temperature, top_k, top_p, min_p, row_seq, row_pos, out)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"sample_rows: x must be (n, V) rows, got {tuple(x.shape)}")
+    n, V = x.shape
+    if x.stride(1) != 1 or (n > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    if u.dtype != torch.float32 or u.dim() != (1 if row_pos is None else 2):
+        raise ValueError("sample_rows: u must be fp32, (entries,) or with row_pos (entries, columns)")
+    entries = u.shape[0]
+    if row_pos is None and u.stride(0) < 1 or row_pos is not None and (u.stride(1) != 1 or u.stride(0) < u.shape[1]):
+        u = u.contiguous()
+    if row_seq is None and entries < n:
+        raise ValueError(f"sample_rows: {n} rows need {n} entries of u")
+    p = _abi.wfd_sample_params()
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None:
+            if t.dtype != dt or t.dim() != 1 or t.shape[0] < entries or not t.is_contiguous():
+                raise ValueError(f"sample_rows: {name} must be a contiguous {dt} vector of {entries} entries")
+            setattr(p, name, t.data_ptr())
+    for name, t in (("row_seq", row_seq), ("row_pos", row_pos)):
+        if t is not None:
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) < 1):
+                raise ValueError(f"sample_rows: {name} must be an int32 vector with one entry per row")
+            setattr(p, name, t.data_ptr())
+            setattr(p, name[4:] + "_stride", max(1, t.stride(0)))
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=dev)
+    elif out.dtype != torch.int32 or tuple(out.shape) != (n,) or not out.is_contiguous():
+        raise ValueError(f"sample_rows: out must be a contiguous int32 vector of {n} entries")
+    p.x, p.out, p.u, p.err = x.data_ptr(), out.data_ptr(), u.data_ptr(), rt.error_word(dev).data_ptr()
+    p.ldx, p.n, p.V, p.dtype = max(V, x.stride(0)), n, V, rt.dtype_code(x.dtype)
+    p.n_params = entries
+    p.u_cols = 1 if u.dim() == 1 else u.shape[1]
+    p.u_stride = max(p.u_cols, u.stride(0))
+    rt.call(dev, "wfd_sample_rows", ctypes.byref(p), rt.stream_ptr(dev))
+    return out
+
 
 # ---------------------------------------------------------------------------
 # skinny linear layers on the tensor cores (wfd_linear): a few rows times a
@@ -176,7 +236,6 @@ def interleave_gate_up(wgu: torch.Tensor) -> torch.Tensor:
 
 def _linear(x: torch.Tensor, w: torch.Tensor, mode: int, *, out=None, norm_eps=None, q=None, k=None, v=None,
             rope=None) -> None:
-    import ctypes
     dev = rt.require_cuda(x, w)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise TypeError("wfd_linear takes bf16 rows and weights")
