@@ -81,3 +81,64 @@ class Q8CacheOracle:
                 out[r0 + j] = np.einsum("hgt,thd->hgd", w, V[:N]).reshape(H, Dh)
                 amp[r0 + j] = np.einsum("hgt,thd->hgd", w, np.abs(V[:N])).reshape(H, Dh)
         return out, amp, smax
+
+
+def decode(W: dict, cfg: dict, prompt: list[int], n_new: int, pick):
+    """Sequential decoding of the looped LM (oracle.looped_lm's architecture) in float64 over an 8-bit cache: the
+    prompt attends its own rows and is cached quantised; every later token attends cached values, its own row
+    included.  pick(logits, position) -> id.  Returns (ids, logits, rows): the logits each id was picked from, and
+    per slot the unquantised (K, V) rows of every position."""
+    import torch
+
+    from oracle import looped_lm as olm
+    H, Hkv, Dh = cfg["n_heads"], cfg["n_kv_heads"], cfg["head_dim"]
+    style = cfg.get("rope_style", "half")
+    n_slots = len(W["prelude"]) + cfg["T_total"] * len(W["core"]) + len(W["coda"])
+    held = [[] for _ in range(n_slots)]      # cached values (K, V), (T, Hkv, Dh)
+    rows = [[] for _ in range(n_slots)]
+
+    def cached(x):
+        q, e = quantise(x.numpy())
+        return torch.from_numpy(q * 2.0 ** e[..., None].astype(np.float64))
+
+    def block(blk, x, slot, pos):
+        T = x.shape[0]
+        h = olm._rms(x, blk["norm1"], cfg["norm_eps"]) @ blk["wqkv"]
+        q, k, v = torch.split(h, [H * Dh, Hkv * Dh, Hkv * Dh], dim=-1)
+        q = olm._rope(q.reshape(T, H, Dh), pos, cfg["rope_theta"], style)
+        k = olm._rope(k.reshape(T, Hkv, Dh), pos, cfg["rope_theta"], style)
+        v = v.reshape(T, Hkv, Dh)
+        rows[slot].append((k, v))
+        held[slot].append((cached(k), cached(v)))
+        if len(held[slot]) > 1:                                    # not the prompt
+            k, v = (torch.cat([t[i] for t in held[slot]]) for i in range(2))
+        k, v = (t.repeat_interleave(H // Hkv, dim=1) for t in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q, k) / np.sqrt(Dh)
+        s = s.masked_fill(torch.arange(k.shape[0])[None, :] > pos[:, None], float("-inf"))
+        o = torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), v).reshape(T, H * Dh)
+        x = x + o @ blk["wo"]
+        g, u = (olm._rms(x, blk["norm2"], cfg["norm_eps"]) @ blk["wgu"]).split(cfg["d_ff"], dim=-1)
+        return x + (torch.nn.functional.silu(g) * u) @ blk["wd"]
+
+    ids, logits = list(prompt), []
+    new = list(prompt)
+    for _ in range(n_new):
+        pos = torch.arange(len(ids) - len(new), len(ids))
+        x = W["embed"][torch.tensor(new)]
+        slot = 0
+        for blk in W["prelude"]:
+            x = block(blk, x, slot, pos)
+            slot += 1
+        e, h = x, torch.zeros_like(x)
+        for _ in range(cfg["T_total"]):
+            h = h + e
+            for blk in W["core"]:
+                h = block(blk, h, slot, pos)
+                slot += 1
+        for blk in W["coda"]:
+            h = block(blk, h, slot, pos)
+            slot += 1
+        logits.append(olm._rms(h[-1], W["final_norm"], cfg["norm_eps"]) @ W["lm_head"])
+        new = [pick(logits[-1], len(ids) - 1)]
+        ids += new
+    return ids[len(prompt):], logits, [tuple(torch.cat([t[i] for t in s]) for i in range(2)) for s in rows]

@@ -83,7 +83,7 @@ class DeviceWave:
         self.tr = _Tables("R", self.r_cap, 6, dev)
         self.tc = _Tables("C", 2 * B, 6 + cfg.n_coda, dev)
         self._params = {}
-        self._graphs: dict[bool, torch.cuda.CUDAGraph] = {}
+        self._graphs: dict[tuple[bool, bool], torch.cuda.CUDAGraph] = {}   # (emulated acceptance, sampled ids)
         self.ticks_replayed = 0
         self.kv_read_bytes = 0
         self.d2h_bytes = 0      # device -> host bytes of the last generate
@@ -155,14 +155,15 @@ class DeviceWave:
         bt = BatchTrace()
         t0 = time.perf_counter()
         _, last_logits = e.prefill(prompt_ids)
-        first = [int(x) for x in last_logits.argmax(dim=-1).tolist()]
+        first = [int(x) for x in e.first_ids(last_logits, int(prompt_ids.shape[1]))]
         torch.cuda.synchronize(self.device)
         bt.prefill_s = time.perf_counter() - t0
         L = int(prompt_ids.shape[1])
         use_emu = emus is not None
         p = self._p(use_emu)
-        if use_graph and use_emu not in self._graphs:
-            self._graphs[use_emu] = self._capture(p)
+        key = (use_emu, e.sampling)
+        if use_graph and key not in self._graphs:
+            self._graphs[key] = self._capture(p)
         # initial state: first token committed, queued for the prelude at position L
         W = self.W
         alive = torch.zeros(B * W, dtype=torch.int32)
@@ -193,7 +194,7 @@ class DeviceWave:
                 em = copy.deepcopy(em)
                 draws[b] = torch.tensor([1 if em.draw() else 0 for _ in range(self.emu_len)], dtype=torch.uint8)
             self.emu.copy_(draws)
-        graph = self._graphs[use_emu] if use_graph else None
+        graph = self._graphs[key] if use_graph else None
 
         guard = self.max_new * (e.cfg.T_total + 4) + 100
         ticks = 0

@@ -27,13 +27,14 @@ ouro_blocks_batch.py:123-248, huginn_blocks_batch.py:207-346), B200-first:
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import numpy as np
 import torch
 
-from . import attention as wa
 from . import fused
 from . import runtime as rt
-from .kv_cache import SlotKVCache
+from .kv_cache import QuantKVCache, SlotKVCache
 from .looped_lm import LoopedLM
 
 _BUCKETS = (8, 16, 32, 64, 128, 256, 512, 1024, 2048)
@@ -97,8 +98,62 @@ class _Tables:
         self.pending = False
 
 
+@dataclass
+class SamplingParams:
+    """How the engine draws ids (fused.sample_rows) in place of the greedy argmax.
+
+    u (batch, max_seq_len): uniform numbers in [0, 1); the row at position p draws
+    the token of position p + 1 with u[b, p], at draft depth and at full depth
+    alike.  A draft is then accepted iff it is the token that full depth draws, so
+    wavefront and draft-then-verify decoding commit the tokens that sequential
+    decoding draws from the same numbers, as they do greedily.  temperature (<= 0:
+    greedy), top_k (0: all), top_p and min_p: one value, or one per sequence."""
+    u: torch.Tensor
+    temperature: float | torch.Tensor = 1.0
+    top_k: int | torch.Tensor = 0
+    top_p: float | torch.Tensor = 1.0
+    min_p: float | torch.Tensor = 0.0
+
+
+class _Sampler:
+    """Device copies of a SamplingParams at fixed addresses (graphs capture them);
+    one more entry, for padding rows, is greedy."""
+
+    def __init__(self, B: int, S: int, device):
+        f32 = dict(dtype=torch.float32, device=device)
+        self.B, self.S = B, S
+        self.u = torch.zeros((B + 1, S), **f32)
+        self.temperature = torch.zeros(B + 1, **f32)
+        self.top_k = torch.zeros(B + 1, dtype=torch.int32, device=device)
+        self.top_p = torch.ones(B + 1, **f32)
+        self.min_p = torch.zeros(B + 1, **f32)
+
+    def load(self, s: SamplingParams) -> None:
+        if tuple(s.u.shape) != (self.B, self.S):
+            raise ValueError(f"SamplingParams.u must be ({self.B}, {self.S}), got {tuple(s.u.shape)}")
+        vals = []
+        for name in ("temperature", "top_k", "top_p", "min_p"):
+            v = torch.as_tensor(getattr(s, name))
+            if v.dim() > 1 or v.dim() == 1 and v.shape[0] != self.B:
+                raise ValueError(f"SamplingParams.{name} must be one value or {self.B}")
+            vals.append((getattr(self, name), v))
+        self.u[:self.B].copy_(s.u)
+        for dst, v in vals:
+            dst[:self.B].copy_(v)
+
+    def draw(self, logits: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None):
+        return fused.sample_rows(logits, self.u, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p,
+                                 min_p=self.min_p, row_seq=seq, row_pos=pos, out=out)
+
+
 class WaveEngine:
-    def __init__(self, model: LoopedLM, batch_size: int, max_seq_len: int, use_graphs: bool = True):
+    """kv_dtype: None keeps K / V in the model's type; "e4m3" in an 8-bit QuantKVCache
+    (the prompt pass attends the prompt's own rows, every tick the cached ones)."""
+
+    def __init__(self, model: LoopedLM, batch_size: int, max_seq_len: int, use_graphs: bool = True,
+                 kv_dtype: str | None = None):
+        if kv_dtype not in (None, "e4m3"):
+            raise ValueError(f"kv_dtype {kv_dtype!r}: None (the model's type) or 'e4m3'")
         cfg = model.cfg
         self.model = model
         self.cfg = cfg
@@ -108,8 +163,11 @@ class WaveEngine:
         self.device = model.device
         self.use_graphs = use_graphs
         # one extra sequence row: the target of padding rows
-        self.cache = SlotKVCache(cfg.n_slots, batch_size + 1, cfg.n_kv_heads, cfg.head_dim, max_seq_len, model.dtype,
-                                 model.device)
+        cache_type = SlotKVCache if kv_dtype is None else QuantKVCache
+        self.cache = cache_type(cfg.n_slots, batch_size + 1, cfg.n_kv_heads, cfg.head_dim, max_seq_len, model.dtype,
+                                model.device)
+        self._sampler: _Sampler | None = None
+        self.sampling = False   # the C unions draw ids (set_sampling) instead of taking the argmax
         self.scratch_seq = batch_size
         # state pool: live tokens are at most B * (T_total / T_draft + 2) per tick;
         # round-robin reuse over this many rows never recycles a live row
@@ -127,7 +185,8 @@ class WaveEngine:
         self.n_launch_calls = 0
         # accounting (host side, exact): K/V bytes the attention of live rows
         # reads, libwfd kernel launches, bytes read back per C union
-        self._row_bytes = cfg.n_kv_heads * cfg.head_dim * torch.finfo(model.dtype).bits // 8
+        self._row_bytes = cfg.n_kv_heads * (cfg.head_dim * torch.finfo(model.dtype).bits // 8 if kv_dtype is None
+                                            else cfg.head_dim + 1)
         # every libwfd kernel a body launches.  Per layer: 2 RMSNorm, RoPE split,
         # plan (with the window append), attention (tcgen05 or CUDA-core), SwiGLU
         # gate.  Per body: P gather + item table + scatter, R gather + item table +
@@ -162,6 +221,30 @@ class WaveEngine:
             for (kind, _), t in self._tables.items():
                 if kind == "R":
                     t.graph = None
+
+    def set_sampling(self, params: SamplingParams | None) -> None:
+        """Draw the ids of later generations with `params`; None: greedy.  New
+        numbers or parameters go into the same buffers, which captured graphs read."""
+        if params is not None:
+            if self._sampler is None:
+                self._sampler = _Sampler(self.B, self.S, self.device)
+            self._sampler.load(params)
+        if (params is not None) != self.sampling:
+            self.sampling = params is not None
+            for (kind, _), t in self._tables.items():
+                if kind == "C":
+                    t.graph = None
+            # the sampled C body runs the final RMSNorm that the folded greedy one leaves out
+            if self.model.fold_norms:
+                self._launches["C"] += 1 if self.sampling else -1
+
+    @torch.no_grad()
+    def first_ids(self, logits: torch.Tensor, prompt_len: int) -> list[int]:
+        """Each sequence's first token from the prompt's last logits (B, V)."""
+        if not self.sampling:
+            return logits.argmax(dim=-1).tolist()
+        seq = torch.arange(self.B, dtype=torch.int32, device=self.device)
+        return self._sampler.draw(logits, seq, torch.full_like(seq, prompt_len - 1)).tolist()
 
     def drop_positions_at_and_after(self, b: int, position: int) -> None:
         self.cache.drop_positions_at_and_after(b, position)
@@ -250,7 +333,7 @@ class WaveEngine:
         before any row attends."""
         m = self.model
         q, k, v = m.qkv(blk, x, pos=t.dev[:, 1])
-        o = wa.wave_attn(q, k, v, self.cache.K, self.cache.V, t.items, 1, lens=self.cache.lens, slot_offset=slot)
+        o = self.cache.wave_attn(q, k, v, t.items, 1, slot_offset=slot)
         return m.finish_block(blk, x, o)
 
     def _body(self, kind: str, t: _Tables) -> None:
@@ -268,8 +351,8 @@ class WaveEngine:
             fused.items_from_table(tab, 4, 3, 1, 5, t.items)   # (slot base, seq, position, live, row)
             for l, blk in enumerate(m.core):
                 q, k, v = m.qkv(blk, x, pos=tab[:, 1])
-                o = wa.wave_attn(q, k, v, self.cache.K, self.cache.V, t.items, self.r_max_q, lens=self.cache.lens,
-                                 slot_offset=cfg.n_prelude + l, row_pos=tab[:, 1] if self.gap_windows else None)
+                o = self.cache.wave_attn(q, k, v, t.items, self.r_max_q, slot_offset=cfg.n_prelude + l,
+                                         row_pos=tab[:, 1] if self.gap_windows else None)
                 x = m.finish_block(blk, x, o)
             fused.scatter_rows(x, rows, self.pool_h)
         else:
@@ -277,7 +360,10 @@ class WaveEngine:
             fused.items_from_table(tab, 4, 3, 1, 5, t.items)
             for j, blk in enumerate(m.coda):
                 x = self._segment_block(blk, x, t, cfg.slot_coda(j))
-            m.greedy_ids(x, t.out)
+            if self.sampling:
+                self._sampler.draw(m.head(x), tab[:, 3], tab[:, 1], t.out)
+            else:
+                m.greedy_ids(x, t.out)
 
     def _run(self, kind: str, t: _Tables) -> None:
         self.n_launch_calls += 1

@@ -201,8 +201,12 @@ class LoopedLM:
             a = fused.silu_mul(self.rmsnorm(x2, blk.norm2) @ blk.wgu)
         return x2.addmm_(a, blk.wd).view(shp)
 
+    def head(self, x: torch.Tensor) -> torch.Tensor:
+        """Logits of the rows x in the model's type (final RMSNorm applied)."""
+        return self.rmsnorm(x.contiguous(), self.final_norm) @ self.lm_head
+
     def logits(self, x: torch.Tensor) -> torch.Tensor:
-        return (self.rmsnorm(x.contiguous(), self.final_norm) @ self.lm_head).float()
+        return self.head(x).float()
 
     def greedy_ids(self, x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """out (int32) = argmax of each row's logits (first maximum), without an fp32 copy.

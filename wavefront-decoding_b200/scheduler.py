@@ -210,10 +210,11 @@ class _Lane:
 
 
 def _start(blocks, prompt_ids, emus, max_new_tokens: int, bt: BatchTrace, t0: float):
-    """Prefill every prompt and commit each sequence's first greedy token
-    (scheduler_batch.py:123-159)."""
+    """Prefill every prompt and commit each sequence's first token: the greedy one
+    (scheduler_batch.py:123-159), or what the blocks' own first_ids draws."""
     cache, logits = blocks.prefill(prompt_ids)
-    first = logits.argmax(dim=-1).tolist()
+    pick = getattr(blocks, "first_ids", None)
+    first = logits.argmax(dim=-1).tolist() if pick is None else pick(logits, int(prompt_ids.shape[1]))
     _synchronize(blocks)
     bt.prefill_s = time.perf_counter() - t0
     L = int(prompt_ids.shape[1])
