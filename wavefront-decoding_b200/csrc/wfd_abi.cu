@@ -1365,27 +1365,36 @@ bool make_q8_map(CUtensorMap* m, const void* base, long long rows, int row_bytes
   cuuint32_t box[3] = {128, 1, (cuuint32_t)box_rows};
   cuuint32_t es[3] = {1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NQP, int NA>
-int launch_q8_tc(const Q8AttnParams& ap, const CUtensorMap& tk, const CUtensorMap& tv, const TailMaps& tails, int sms,
-                 cudaStream_t st) {
-  using C = Q8Cfg<NQP>;
+template <int NQP, int NA, bool PAIR>
+int launch_q8_tc(const Q8AttnParams& ap, const Q8Maps& maps, int sms, cudaStream_t st) {
+  using C = Q8Cfg<NQP, q8_groups(NA)>;
   static std::atomic<bool> attr_set[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WFD_ERR_CUDA;
   if (!attr_set[dev].load()) {
-    if (cudaFuncSetAttribute(q8_tc_kernel<NQP, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
+    if (cudaFuncSetAttribute(q8_tc_kernel<NQP, NA, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
         cudaSuccess)
       return WFD_ERR_CUDA;
     attr_set[dev].store(true);
   }
-  return launch_pdl(q8_tc_kernel<NQP, NA>, dim3(sms), dim3(q8_tc_threads(NA)), C::SMEM, st, tk, tv, tails, ap) ==
+  return launch_pdl(q8_tc_kernel<NQP, NA, PAIR>, dim3(sms), dim3(q8_tc_threads(NA)), C::SMEM, st, maps, ap) ==
                  cudaSuccess
              ? WFD_OK
              : WFD_ERR_CUDA;
+}
+
+// nv: query vectors of a unit, at most
+template <bool PAIR>
+int launch_q8_cols(long long nv, const Q8AttnParams& ap, const Q8Maps& maps, int sms, cudaStream_t st) {
+  if (nv <= 2) return launch_q8_tc<16, 2, PAIR>(ap, maps, sms, st);
+  if (nv <= 4) return launch_q8_tc<16, 4, PAIR>(ap, maps, sms, st);
+  if (nv <= 8) return launch_q8_tc<16, 8, PAIR>(ap, maps, sms, st);
+  if (nv <= 16) return launch_q8_tc<16, 16, PAIR>(ap, maps, sms, st);
+  return launch_q8_tc<32, 32, PAIR>(ap, maps, sms, st);
 }
 
 template <typename T, int DH>
@@ -1542,15 +1551,11 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   static_assert(2 * kQ8SimtNQ * (128 + 2) <= 2 * kVerifyMaxRows * (128 + 2), "partials of the CUDA-core kernel");
   const bool invariant = g_batch_invariant.load(std::memory_order_relaxed) != 0;
   const bool self_plan = which == 1 && n_items <= kSelfPlanMax;
-  CUtensorMap tk, tv;
-  TailMaps tails;
+  Q8Maps maps;
   if (which == 1) {
-    const int rb = c.Hkv * Dh;
-    if (!make_q8_map(&tk, cache->k, key_rows, rb, kTcTile) || !make_q8_map(&tv, cache->v, key_rows, rb, kTcTile))
-      return WFD_ERR_CUDA;
-    for (int pc = 0; pc < 4; ++pc)
-      if (!make_q8_map(&tails.k[pc], cache->k, key_rows, rb, 64 >> pc) ||
-          !make_q8_map(&tails.v[pc], cache->v, key_rows, rb, 64 >> pc))
+    for (int i = 0; i < kQ8Boxes; ++i)
+      if (!make_q8_map(&maps.k[i], cache->k, key_rows, c.Hkv * Dh, 256 >> i) ||
+          !make_q8_map(&maps.v[i], cache->v, key_rows, c.Hkv * Dh, 256 >> i))
         return WFD_ERR_CUDA;
   }
 
@@ -1583,6 +1588,7 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   pp.q8 = c;
   pp.zero = reinterpret_cast<int*>(ws + L.cnt);
   pp.n_zero = sms;
+  pp.min_share = kQ8MinShare;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 plan_grid(1 + (n_items < 4 * sms ? n_items : 4 * sms));
   const cudaError_t pe = dtype == WFD_DTYPE_BF16
@@ -1628,11 +1634,7 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
     ap.Gv = Gv;
     ap.NQ = NQ;
   }
-  if (NQ == 32) return launch_q8_tc<32, 32>(ap, tk, tv, tails, sms, st);
-  if (nv <= 2) return launch_q8_tc<16, 2>(ap, tk, tv, tails, sms, st);
-  if (nv <= 4) return launch_q8_tc<16, 4>(ap, tk, tv, tails, sms, st);
-  if (nv <= 8) return launch_q8_tc<16, 8>(ap, tk, tv, tails, sms, st);
-  return launch_q8_tc<16, 16>(ap, tk, tv, tails, sms, st);
+  return pair ? launch_q8_cols<true>(nv, ap, maps, sms, st) : launch_q8_cols<false>(nv, ap, maps, sms, st);
 }
 
 // ---------------------------------------------------------------------------

@@ -66,6 +66,7 @@ struct PlanParams {
   // window append into an 8-bit cache (plan_kernel<T>: k_new / v_new hold T rows);
   // its slots and the items' are both counted from the call's slot offset
   Q8Cache q8;
+  int min_share;  // plan_kernel<T>: smallest share of a CTA (0: none)
   int* zero;  // plan_kernel<T>: arrival counters cleared for the attention (n_zero)
   int n_zero;
 };
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   if (p.start != nullptr) {
     __syncthreads();  // the prefix above is complete and visible to the block
     const long long total = (long long)p.seg_units * carry;
-    const long long share = total > 0 ? (total + p.seg_grid - 1) / p.seg_grid : 1;
+    long long share = total > 0 ? (total + p.seg_grid - 1) / p.seg_grid : 1;
+    if constexpr (!std::is_void<TQ>::value) share = share < p.min_share ? p.min_share : share;
     const long long* pf = staged ? s_prefix : p.prefix;
     for (int c = threadIdx.x; c < p.seg_grid; c += blockDim.x) {
       const long long a = (long long)c * share;

@@ -26,6 +26,11 @@ struct Q8AttnParams : VerifyParams {
   Q8Cache c;  // counted from the call's slot offset
 };
 
+// A CTA's share is at least this many keys of one unit: a piece of fewer takes as
+// long as a whole tile pair of the tensor-core kernel, and every further piece is
+// one more to merge.
+constexpr int kQ8MinShare = 256;
+
 constexpr int kQ8SimtThreads = 384;
 constexpr int kQ8SimtNQ = 4;  // query vectors per unit, at most
 
@@ -48,7 +53,7 @@ __global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8Attn
   const long long total = (long long)p.Hkv * p.prefix[p.n_segs];
   long long share = 1, a = 0, b = 0;
   if (total > 0) {
-    share = (total + gridDim.x - 1) / gridDim.x;
+    share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
     a = (long long)blockIdx.x * share;
     b = (a + share < total) ? a + share : total;
   }

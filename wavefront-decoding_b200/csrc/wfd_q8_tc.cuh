@@ -31,8 +31,8 @@
 // the chain's latency is paid once per 64 KB, as in the bf16 kernel.
 //
 // Warp roles (one CTA per SM): 0 TMA producer; 1 TMEM owner and MMA issuer; 2 the
-// Q operand of the next units (two buffers); 3.. softmax, 4 warps per slice of the
-// query columns.  Work split, merging and the self-planned start are K2's
+// Q operand of the next units (two buffers); 3 the keys' exponents (a ring of tile
+// pairs); 4.. softmax, 4 warps per slice of the query columns.  Work split, merging and the self-planned start are K2's
 // (UnitIter, CtaStart).  Every wait is bounded; no multicast, no cluster.
 #pragma once
 
@@ -40,30 +40,53 @@
 
 namespace wfd {
 
-template <int NQP>
+// Tensor maps of a code buffer: boxes of 256 rows (a tile pair), and of 128, 64, 32,
+// 16 and 8 for its tail.
+constexpr int kQ8Boxes = 6;
+struct Q8Maps {
+  CUtensorMap k[kQ8Boxes];
+  CUtensorMap v[kQ8Boxes];
+};
+
+template <int NQP, int G>
 struct Q8Cfg {
   static constexpr int N = 2 * NQP;                  // MMA columns: both pieces
-  static constexpr int STAGES = NQP == 16 ? 6 : 5;   // 128-key tiles of K and V
+  // Rings of tile pairs (256 keys x 128 bytes).  A K pair is done with after S, a V
+  // pair only after the softmax and P.V, one pair later: twice the V pairs keep as
+  // many of either in flight.
+  static constexpr int KS = 2;
+  static constexpr int VS = NQP == 16 ? 4 : 3;
   static constexpr int TILE_BYTES = kTcTile * 128;
-  static constexpr int KV_STAGE = 2 * TILE_BYTES;
+  static constexpr int PAIR_BYTES = 2 * TILE_BYTES;
   static constexpr int Q_BYTES = N * 128;            // one of two buffers
   static constexpr int P_ROWB = N;                   // one key's row of P^T
-  static constexpr int P_BYTES = 2 * kTcTile * P_ROWB;
+  static constexpr int P_BYTES = 2 * kTcTile * P_ROWB;     // one group's
   static constexpr int P_SWZ_BITS = NQP == 16 ? 1 : 2;     // 32- / 64-byte swizzle
   static constexpr uint64_t P_LAYOUT = NQP == 16 ? 6 : 4;
   static constexpr int P_ATOM = 8 * P_ROWB;
-  static constexpr int RED_FLOATS = 2 * 4 * NQP;
-  static constexpr int SMEM = STAGES * KV_STAGE + 2 * Q_BYTES + P_BYTES + 2 * RED_FLOATS * 4 + 4 * NQP * 4 + 1024;
+  static constexpr int RED_FLOATS = G * 2 * 4 * NQP;
+  static constexpr int EXP_RING = 4;                 // tile pairs of key / value exponents, one 32-bit word a key
+  static constexpr int EXP_BYTES = EXP_RING * 2 * kTcTile * 4;
+  static constexpr int MX_FLOATS = (NQP == 16 ? 8 : 16) * 2 * 16;  // per softmax warp: running maxima and rescale factors
+  static constexpr int ML_FLOATS = 2 * NQP;          // the second group's maxima and sums at the end of a unit
+  static constexpr int SMEM = (KS + VS) * PAIR_BYTES + 2 * Q_BYTES + G * P_BYTES + EXP_BYTES +
+                              (2 * RED_FLOATS + 4 * NQP + MX_FLOATS + ML_FLOATS) * 4 + 1024;
   static constexpr int S_COL = 0;                    // S^T of tile pair buffer sb, half hf: (2 sb + hf) N
-  static constexpr int O_COL = 4 * N;                // O^T, two accumulator chains
+  static constexpr int O_COL = 4 * N;                // O^T of group g: O_COL + g N
   static constexpr int TMEM_COLS = NQP == 16 ? 256 : 512;
   static constexpr int PART_FLOATS = NQP * (128 + 2);
-  static_assert(O_COL + 2 * N <= TMEM_COLS, "TMEM columns");
+  static_assert(O_COL + G * N <= TMEM_COLS, "TMEM columns");
   static_assert(SMEM + 2048 <= 232448, "shared memory per CTA (dynamic + the kernel's static arrays)");
 };
 
-__host__ __device__ constexpr int q8_slices(int na) { return na >= 16 ? 2 : 1; }  // column slices of the softmax
-__host__ __device__ constexpr int q8_tc_threads(int na) { return 96 + 128 * q8_slices(na); }
+// Softmax warps: groups that take alternate tile pairs, each with its own maxima,
+// sums and O (merged at the end of a unit), and slices of the query columns inside
+// a group.  Up to 16 columns a pair's softmax is a chain of dependent steps, and two
+// groups keep two pairs in it; 32 columns are bound by instruction issue, and four
+// slices of 8 fill the schedulers with less state a thread.
+__host__ __device__ constexpr int q8_groups(int na) { return na <= 16 ? 2 : 1; }
+__host__ __device__ constexpr int q8_slices(int na) { return na <= 16 ? 1 : na / 8; }
+__host__ __device__ constexpr int q8_tc_threads(int na) { return 128 + 128 * q8_groups(na) * q8_slices(na); }
 
 // kind::f8f6f4, e4m3 x e4m3 -> f32, M = 128
 __host__ __device__ constexpr uint32_t q8_idesc(int n, bool a_mn_major, bool b_mn_major) {
@@ -77,6 +100,35 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+// A value every lane holds, known to the compiler as warp-uniform: tcgen05.mma takes
+// its operands in uniform registers, and moving them there from per-thread ones
+// made the issue of one MMA cost 154 cycles against 41 (of which 32 are the reads
+// of the A operand).
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// One lane of the (converged) warp, the same at every call.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Bounded mbarrier wait by every lane of a warp, with a warp-uniform result: one
+// probe and one vote when the phase has completed (every pair passes about ten of
+// these; tc_wait's further load of the abort flag made them 200 cycles each).
+// Otherwise it gives up at the spin limit (error word and CTA abort flag) or as soon
+// as another role has aborted: the roles keep their control flow, issue no more
+// work that depends on the wait, and every wait after it ends the same way.
+__device__ __forceinline__ bool q8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  for (uint32_t i = 1; i < kSpinLimit; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  set_error(err, kErrTimeout);
+  *abort_flag = 1;
+  return false;
 }
 
 // 32 TMEM lanes, N consecutive columns -> N registers per thread
@@ -101,12 +153,48 @@ __device__ __forceinline__ void tmem_cols(uint32_t taddr, float (&v)[N]) {
   }
 }
 
-// Two weights as two pieces: codes of (a, b) in the low 16 bits of p1 and p2.
-__device__ __forceinline__ void q8_split(float a, float b, uint32_t& p1, uint32_t& p2) {
+// Two fp32 values in one 64-bit register: one instruction for both (the softmax of
+// 32 columns is bound by instruction issue).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void up2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x, 0 far below; x <= 9 here (a NaN stays one)
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two values as two pieces: codes of (a, b) in the low 16 bits of p1 and p2.
+__device__ __forceinline__ void q8_split(f32x2 w, uint32_t& p1, uint32_t& p2) {
+  float a, b;
+  up2(w, a, b);
   p1 = e4m3x2(a, b);
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)p1, __NV_E4M3);
   const float2 f = __half22float2(__half2(h));
-  p2 = e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f);
+  const f32x2 r = fma2(pk2(f.x, f.y), pk2(-16.f, -16.f), mul2(w, pk2(16.f, 16.f)));  // 16 (w - f), exact
+  up2(r, a, b);
+  p2 = e4m3x2(a, b);
 }
 
 // A CTA's share of the work and where it starts, from the item table itself (K2's
@@ -154,7 +242,7 @@ __device__ __forceinline__ long long self_start(const VerifyParams& p, SelfStart
   share = 1;
   a = b = 0;
   if (total > 0) {
-    share = (total + gridDim.x - 1) / gridDim.x;
+    share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
     a = (long long)blockIdx.x * share;
     b = (a + share < total) ? a + share : total;
   }
@@ -188,79 +276,95 @@ __device__ __forceinline__ long long self_start(const VerifyParams& p, SelfStart
 
 // The query columns of one unit: up to NQP vectors of one kv head, or up to NQP / 2
 // of either head of a pair (head 0's first).
+template <bool PAIR, int NQP>
 struct UnitCols {
   int v0, nv1, nvec;
-  __device__ __forceinline__ UnitCols(const VerifyParams& p, const Seg& S, int qg, int nqp) {
-    const int gh = p.pair ? nqp / 2 : nqp;
+  __device__ __forceinline__ UnitCols(const VerifyParams& p, const Seg& S, int qg) {
+    constexpr int gh = PAIR ? NQP / 2 : NQP;
     v0 = qg * gh;
     nv1 = min(gh, S.q_len * p.G - v0);
-    nvec = p.pair ? 2 * nv1 : nv1;
-    if (!p.pair) nv1 = 0x7fffffff;
+    nvec = PAIR ? 2 * nv1 : nv1;
   }
-  __device__ __forceinline__ int head(int n) const { return n >= nv1 ? 1 : 0; }
-  __device__ __forceinline__ int vec(int n) const { return v0 + (n >= nv1 ? n - nv1 : n); }
+  __device__ __forceinline__ int head(int n) const { return PAIR && n >= nv1 ? 1 : 0; }
+  __device__ __forceinline__ int vec(int n) const { return v0 + (PAIR && n >= nv1 ? n - nv1 : n); }
 };
 
 // NA: query columns the softmax works on (every unit has at most NA vectors).
-template <int NQP, int NA>
+template <int NQP, int NA, bool PAIR>
 __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
-    q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ TailMaps tails, const Q8AttnParams p) {
-  using C = Q8Cfg<NQP>;
-  constexpr int STAGES = C::STAGES;
+    q8_tc_kernel(const __grid_constant__ Q8Maps maps, const Q8AttnParams p) {
+  constexpr int G = q8_groups(NA);   // softmax groups
+  constexpr int H = q8_slices(NA);   // column slices of a group (4 warps each)
+  using C = Q8Cfg<NQP, G>;
+  constexpr int KS = C::KS, VS = C::VS;
   constexpr int N = C::N;
   constexpr int THREADS = q8_tc_threads(NA);
-  constexpr int H2 = q8_slices(NA);  // column slices of the softmax (4 warps each)
-  constexpr int NL = NA / H2;        // query columns per softmax thread
-  constexpr int SMT = 128 * H2;
+  constexpr int NL = NA / H;         // query columns per softmax thread
+  constexpr int SMT = 128 * H;       // softmax threads of a group
+  static_assert(4 * G * H * 32 <= C::MX_FLOATS && (G == 1 || NL * kTcTile * 4 <= C::P_BYTES), "the merge of two groups");
   static_assert(NL == 2 || NL == 4 || NL == 8 || NL == 16, "columns per softmax thread");
   static_assert(NA <= NQP, "active query columns");
+  static_assert(KS == 2, "the K ring shares S's barriers");
   const float NEG_INF = -__int_as_float(0x7f800000);
 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* kvs = smem;                                // STAGES x (K tile, V tile)
-  unsigned char* qs = kvs + STAGES * C::KV_STAGE;           // 2 x Q operand (K-major, 128B swizzle)
-  unsigned char* ps = qs + 2 * C::Q_BYTES;                  // P^T operand of a tile pair (MN-major)
-  float* red = reinterpret_cast<float*>(ps + C::P_BYTES);   // [2][4][NQP] column maxima
-  float* lred = red + C::RED_FLOATS;                        // [2][4][NQP] column sums
-  float* cscale = lred + C::RED_FLOATS;                     // [4][NQP] score scale of each column, per unit
+  unsigned char* kts = smem;                                // KS K tile pairs
+  unsigned char* vts = kts + KS * C::PAIR_BYTES;            // VS V tile pairs
+  unsigned char* qs = vts + VS * C::PAIR_BYTES;             // 2 x Q operand (K-major, 128B swizzle)
+  unsigned char* ps = qs + 2 * C::Q_BYTES;                  // P^T operand of a tile pair (MN-major), per group
+  float* red = reinterpret_cast<float*>(ps + G * C::P_BYTES);  // [G][2][4][NQP] column maxima
+  float* lred = red + C::RED_FLOATS;                        // [G][2][4][NQP] column sums
+  float* ml = lred + C::RED_FLOATS;                         // [2][NQP] the second group's maxima and sums
+  float* cscale = ml + C::ML_FLOATS;                     // [4][NQP] score scale of each column, per unit
+  float* mxs = cscale + 4 * NQP;                            // [16][2][16] per softmax warp
+  uint32_t* exps = reinterpret_cast<uint32_t*>(mxs + C::MX_FLOATS);  // [EXP_RING][2][128] exponents of a key
 
-  __shared__ __align__(8) uint64_t bar_full[STAGES];
-  __shared__ __align__(8) uint64_t bar_empty[STAGES];
+  __shared__ __align__(8) uint64_t bar_kfull[KS];
+  __shared__ __align__(8) uint64_t bar_vfull[VS];
+  __shared__ __align__(8) uint64_t bar_vempty[VS];
   __shared__ __align__(8) uint64_t bar_sfull[2];
   __shared__ __align__(8) uint64_t bar_sfree[2];
-  __shared__ __align__(8) uint64_t bar_pfull;
-  __shared__ __align__(8) uint64_t bar_ofull;
-  __shared__ __align__(8) uint64_t bar_ofree;
+  __shared__ __align__(8) uint64_t bar_pfull[G];
+  __shared__ __align__(8) uint64_t bar_ofull[G];
   __shared__ __align__(8) uint64_t bar_qready[4];  // unit's Q and column scales written
   __shared__ __align__(8) uint64_t bar_qfree[2];
   __shared__ __align__(8) uint64_t bar_drain;
+  __shared__ __align__(8) uint64_t bar_efull[C::EXP_RING];   // a tile pair's exponents written
+  __shared__ __align__(8) uint64_t bar_efree[C::EXP_RING];   // ... and read by every softmax warp
   __shared__ uint32_t s_tmem;
-  __shared__ int s_rp[NQP];  // gapped windows: each query column's row position
+  __shared__ int s_rp[G][NQP];  // gapped windows: each query column's row position
   __shared__ volatile int s_abort;
   __shared__ int s_flag;
   __shared__ SelfStart s_start;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = (int)uniform((uint32_t)tid >> 5), lane = tid & 31;
   const bool self = p.items != nullptr;
   if (tid == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&bar_full[s], 1);
-      mbar_init(&bar_empty[s], 1);
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k[0])) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v[0])) : "memory");
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&bar_kfull[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(&bar_vfull[s], 1);
+      mbar_init(&bar_vempty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar_sfull[s], 1);
-      mbar_init(&bar_sfree[s], 4 * H2);
+      mbar_init(&bar_sfree[s], 4 * H);
       mbar_init(&bar_qfree[s], 1);
     }
     for (int s = 0; s < 4; ++s) mbar_init(&bar_qready[s], 1);
-    mbar_init(&bar_pfull, 1);
-    mbar_init(&bar_ofull, 1);
-    mbar_init(&bar_ofree, 4 * H2);
+    for (int s = 0; s < C::EXP_RING; ++s) {
+      mbar_init(&bar_efull[s], 1);
+      mbar_init(&bar_efree[s], 4 * H);
+    }
+    for (int s = 0; s < G; ++s) {
+      mbar_init(&bar_pfull[s], 1);
+      mbar_init(&bar_ofull[s], 1);
+    }
     mbar_init(&bar_drain, 1);
     fence_mbar_init();
     s_abort = 0;
@@ -291,7 +395,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
     cs = p.start[blockIdx.x];
     const long long total = (long long)p.Hkv * p.prefix[p.n_segs];
     if (total > 0) {
-      share = (total + gridDim.x - 1) / gridDim.x;
+      share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
       a = (long long)blockIdx.x * share;
       b = (a + share < total) ? a + share : total;
     }
@@ -324,124 +428,160 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
     // ------------------------------------------------------------ TMA producer
     UnitIter itr = make_iter();
     uint32_t it = 0;
-    uint32_t n_iss = 0;  // tiles whose loads were issued (a prefix of the sequence: issue stops at an abort)
+    uint32_t n_k = 0, n_v = 0;  // pairs whose loads were issued (prefixes of the sequence: issue stops at an abort)
     while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
       const int h = u % p.Hkv;
-      const int n_sub = (r_hi - r_lo + kTcTile - 1) / kTcTile;
+      const int n_t = (r_hi - r_lo + 2 * kTcTile - 1) / (2 * kTcTile);
       const long long row0 = S.k_row0 + p.k_row_offset + r_lo;
-      for (int t = 0; t < n_sub; ++t, ++it) {
-        const int stage = (int)(it % STAGES);
-        need_rows(itr, r_lo + (t + 1) * kTcTile);
-        const bool go = (it >= (uint32_t)STAGES) ? tc_wait(&bar_empty[stage], ((it / STAGES) - 1) & 1u, &s_abort, p.err)
-                                                 : !s_abort;
-        if (go && lane == 0) {
-          unsigned char* dst = kvs + stage * C::KV_STAGE;
-          const int row = (int)(row0 + (long long)t * kTcTile);
-          // a tail of at most 96 rows loads only those, in pieces of 64 / 32 / 16 / 8
-          const int rows_left = r_hi - r_lo - t * kTcTile;
-          const int nr = rows_left > 96 ? kTcTile : ((rows_left + 7) & ~7);
-          mbar_arrive_expect_tx(&bar_full[stage], (uint32_t)(nr * 128 * 2));
-          if (nr == kTcTile) {
-            tma_load_3d(dst, &tm_k, 0, h, row, &bar_full[stage]);
-            tma_load_3d(dst + C::TILE_BYTES, &tm_v, 0, h, row, &bar_full[stage]);
+      for (int t = 0; t < n_t; ++t, ++it) {
+        need_rows(itr, r_lo + (t + 1) * 2 * kTcTile);
+        const int row = (int)(row0 + (long long)t * 2 * kTcTile);
+        // a last pair of at most 224 keys loads only those, in boxes of 128 / 64 / 32 /
+        // 16 / 8 rows; what the stage holds past them is masked (V: zeroed)
+        const int left = r_hi - r_lo - t * 2 * kTcTile;
+        const int nr = left > 224 ? 2 * kTcTile : ((left + 7) & ~7);
+        auto load = [&](unsigned char* dst, const CUtensorMap* m, uint64_t* bar) {
+          mbar_arrive_expect_tx(bar, (uint32_t)(nr * 128));
+          if (nr == 2 * kTcTile) {
+            tma_load_3d(dst, m, 0, h, row, bar);
           } else {
             int off = 0;
-#pragma unroll
-            for (int pc = 0; pc < 4; ++pc) {
-              const int pr = 64 >> pc;
+            for (int pc = 1; pc < kQ8Boxes; ++pc) {
+              const int pr = 256 >> pc;
               if (nr & pr) {
-                tma_load_3d(dst + off * 128, &tails.k[pc], 0, h, row + off, &bar_full[stage]);
-                tma_load_3d(dst + C::TILE_BYTES + off * 128, &tails.v[pc], 0, h, row + off, &bar_full[stage]);
+                tma_load_3d(dst + off * 128, m + pc, 0, h, row + off, bar);
                 off += pr;
               }
             }
           }
-          n_iss = it + 1;
-          if (p.fail_waits && n_iss == 1) {  // test hook: give up with this tile's copies in flight
+        };
+        const int ks = (int)(it % KS), vs = (int)(it % VS);
+        // (the K ring is as deep as S: pair it - 2's S complete frees its K)
+        bool go = it >= (uint32_t)KS ? q8_wait(&bar_sfull[ks], ((it / KS) - 1) & 1u, &s_abort, p.err) : !s_abort;
+        if (go && lane == 0) {
+          load(kts + ks * C::PAIR_BYTES, maps.k, &bar_kfull[ks]);
+          n_k = it + 1;
+          if (p.fail_waits && n_k == 1) {  // test hook: give up with this copy in flight
             set_error(p.err, kErrTimeout);
             s_abort = 1;
           }
         }
         __syncwarp();
+        go = it >= (uint32_t)VS ? q8_wait(&bar_vempty[vs], ((it / VS) - 1) & 1u, &s_abort, p.err) : !s_abort;
+        if (go && lane == 0) {
+          load(vts + vs * C::PAIR_BYTES, maps.v, &bar_vfull[vs]);
+          n_v = it + 1;
+        }
+        __syncwarp();
       }
     }
-    const uint32_t n_used = it;
-    for (uint32_t j = (n_used > (uint32_t)STAGES ? n_used - STAGES : 0); j < n_used; ++j)
-      tc_wait(&bar_empty[j % STAGES], (j / STAGES) & 1u, &s_abort, p.err);
+    // the MMA warp's commits land on these barriers before the CTA exits
+    for (uint32_t j = (it > (uint32_t)VS ? it - VS : 0); j < it; ++j)
+      q8_wait(&bar_vempty[j % VS], (j / VS) & 1u, &s_abort, p.err);
     // copies in flight land before the CTA exits, also after an abort
     if (lane == 0) {
-      for (uint32_t j = (n_iss > (uint32_t)STAGES ? n_iss - STAGES : 0); j < n_iss; ++j)
-        if (!mbar_wait_bounded(&bar_full[j % STAGES], (j / STAGES) & 1u)) set_error(p.err, kErrTimeout);
+      for (uint32_t j = (n_k > (uint32_t)KS ? n_k - KS : 0); j < n_k; ++j)
+        if (!mbar_wait_bounded(&bar_kfull[j % KS], (j / KS) & 1u)) set_error(p.err, kErrTimeout);
+      for (uint32_t j = (n_v > (uint32_t)VS ? n_v - VS : 0); j < n_v; ++j)
+        if (!mbar_wait_bounded(&bar_vfull[j % VS], (j / VS) & 1u)) set_error(p.err, kErrTimeout);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     UnitIter itr = make_iter();
-    uint32_t it = 0, tt = 0, pv = 0, units = 0;
+    uint32_t it = 0, units = 0;  // it: tile pairs before this unit
     constexpr uint32_t IDESC_S = q8_idesc(N, false, false);
     constexpr uint32_t IDESC_PV = q8_idesc(N, true, true);
     const uint32_t q_addr = smem_u32(qs);
     const uint32_t p_addr = smem_u32(ps);
+    const uint32_t k_addr = smem_u32(kts);
+    const uint32_t v_addr = smem_u32(vts);
+    const uint32_t tm = uniform(tmem);
     while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
       const int n_sub = (r_hi - r_lo + kTcTile - 1) / kTcTile;
       const int n_t = (n_sub + 1) >> 1;
       const int qb = (int)(units & 1u);
-      const uint32_t qa = q_addr + (uint32_t)(qb * C::Q_BYTES);
-      tc_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
+      const uint32_t qa = uniform(q_addr + (uint32_t)(qb * C::Q_BYTES));
+      q8_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
       tc_fence_after();
-      for (int t = 0; t <= n_t; ++t) {
-        if (t < n_t) {
-          const uint32_t ti = tt + t;
-          const int sb = (int)(ti & 1u);
-          const int nh = (2 * t + 1 < n_sub) ? 2 : 1;
-          const uint32_t i0 = it + 2 * t;
-          bool go = true;
-          for (int hf = 0; hf < nh; ++hf)
-            go = tc_wait(&bar_full[(i0 + hf) % STAGES], ((i0 + hf) / STAGES) & 1u, &s_abort, p.err) && go;
-          if (ti >= 2) go = tc_wait(&bar_sfree[sb], ((ti >> 1) - 1) & 1u, &s_abort, p.err) && go;
+      // S of pair t + 1 goes out before P.V of pair t, whose weights the softmax is
+      // still computing; but when its keys are late, P.V does not wait for them
+      int ts = 0, tv = 0;
+      while (tv < n_t) {
+        bool do_s = ts < n_t, s_ok = false, p_ok = false;
+        if (do_s && tv < ts) {
+          const uint32_t i = it + ts, j = it + tv;
+          for (uint32_t n = 0; n < kSpinLimit; ++n) {  // (every exit by a vote)
+            s_ok = __all_sync(0xffffffffu, mbar_test_wait(&bar_kfull[i % KS], (i / KS) & 1u) &&
+                                               (i < 2 || mbar_test_wait(&bar_sfree[i & 1u], ((i >> 1) - 1) & 1u)));
+            if (s_ok) break;
+            p_ok = __all_sync(0xffffffffu, mbar_test_wait(&bar_pfull[j % G], (j / G) & 1u));
+            if (p_ok || __any_sync(0xffffffffu, s_abort != 0)) break;
+          }
+          do_s = !p_ok;
+        }
+        if (do_s) {
+          const uint32_t i = it + ts;
+          const int sb = (int)(i & 1u), ks = (int)(i % KS);
+          const bool two = uniform(2 * ts + 1 < n_sub) != 0;
+          bool go = s_ok;
+          if (!s_ok) {
+            go = q8_wait(&bar_kfull[ks], (i / KS) & 1u, &s_abort, p.err);
+            if (i >= 2) go = q8_wait(&bar_sfree[sb], ((i >> 1) - 1) & 1u, &s_abort, p.err) && go;
+          }
           tc_fence_after();
-          if (go && lane == 0) {
+          const uint32_t k0 = uniform(k_addr + (uint32_t)(ks * C::PAIR_BYTES));
+          const uint32_t d0 = uniform(tm + (uint32_t)(2 * sb * N));
+          if (go && elect_lane()) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // 32 bytes of the row; the halves are independent accumulators
-              for (int hf = 0; hf < nh; ++hf) {
-                const uint32_t k_addr = smem_u32(kvs + (int)((i0 + hf) % STAGES) * C::KV_STAGE);
-                umma_f8(tmem + (uint32_t)((2 * sb + hf) * N), umma_desc(k_addr + j * 32, 16, 1024, 2),
+            for (int j = 0; j < 4; ++j) {  // 32 bytes of the row; the two tiles are independent accumulators
+              umma_f8(d0, umma_desc(k0 + j * 32, 16, 1024, 2), umma_desc(qa + j * 32, 16, 1024, 2), IDESC_S,
+                      j > 0 ? 1u : 0u);
+              if (two)
+                umma_f8(d0 + N, umma_desc(k0 + C::TILE_BYTES + j * 32, 16, 1024, 2),
                         umma_desc(qa + j * 32, 16, 1024, 2), IDESC_S, j > 0 ? 1u : 0u);
-              }
             }
             umma_commit(&bar_sfull[sb]);
-            if (t == n_t - 1) umma_commit(&bar_qfree[qb]);  // the unit's Q buffer may be rewritten
+            if (ts == n_t - 1) umma_commit(&bar_qfree[qb]);  // the unit's Q buffer may be rewritten
           }
           __syncwarp();
-        }
-        if (t >= 1) {
-          bool go = tc_wait(&bar_pfull, pv & 1u, &s_abort, p.err);
-          if (pv >= 1) go = tc_wait(&bar_ofree, (pv - 1) & 1u, &s_abort, p.err) && go;
+          ++ts;
+        } else {
+          const uint32_t i = it + tv;
+          const int vs = (int)(i % VS);
+          const bool two = uniform(2 * tv + 1 < n_sub) != 0;
+          bool go = q8_wait(&bar_vfull[vs], (i / VS) & 1u, &s_abort, p.err);
+          const int g = (int)(i % G);
+          // (P of pair i written: the group has read S and the O of its pair before)
+          if (!p_ok) go = q8_wait(&bar_pfull[g], (i / G) & 1u, &s_abort, p.err) && go;
           tc_fence_after();
-          const int nh = (2 * (t - 1) + 1 < n_sub) ? 2 : 1;
-          const uint32_t i0 = it + 2 * (t - 1);
-          if (go && lane == 0) {
-            for (int hf = 0; hf < nh; ++hf) {
-              const uint32_t v_addr = smem_u32(kvs + (int)((i0 + hf) % STAGES) * C::KV_STAGE + C::TILE_BYTES);
+          const uint32_t v0 = uniform(v_addr + (uint32_t)(vs * C::PAIR_BYTES));
+          const uint32_t o0 = uniform(tm + (uint32_t)(C::O_COL + g * N));
+          const uint32_t p0 = uniform(p_addr + (uint32_t)(g * C::P_BYTES));
+          if (go && elect_lane()) {
+            // k-step j: 32 keys, four 8-row groups of V and of P^T
 #pragma unroll
-              for (int j = 0; j < 4; ++j)  // 32 keys: four 8-row groups of V and of P^T
-                umma_f8(tmem + (uint32_t)(C::O_COL + (j & 1) * N), umma_desc(v_addr + j * 4096, 16, 1024, 2),
-                        umma_desc(p_addr + (hf * 16 + j * 4) * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV,
-                        (hf > 0 || j >= 2) ? 1u : 0u);
+            for (int j = 0; j < 4; ++j)
+              umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
+                      umma_desc(p0 + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, j > 0 ? 1u : 0u);
+            if (two) {
+#pragma unroll
+              for (int j = 4; j < 8; ++j)
+                umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
+                        umma_desc(p0 + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, 1u);
             }
-            umma_commit(&bar_ofull);
-            for (int hf = 0; hf < nh; ++hf) umma_commit(&bar_empty[(i0 + hf) % STAGES]);
+            umma_commit(&bar_ofull[g]);
+            umma_commit(&bar_vempty[vs]);
           }
           __syncwarp();
-          ++pv;
+          ++tv;
         }
       }
-      it += n_sub;
-      tt += n_t;
+      it += n_t;
       ++units;
     }
     // every MMA complete before TMEM is freed and the CTA exits, also after an abort
-    if (lane == 0) {
+    if (elect_lane()) {
       umma_commit(&bar_drain);
       if (!mbar_wait_bounded(&bar_drain, 0)) set_error(p.err, kErrTimeout);
     }
@@ -458,9 +598,9 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
     while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
       const int h = u % p.Hkv, qg = u / p.Hkv;
       const int qb = (int)(units & 1u);
-      const bool go = units >= 2 ? tc_wait(&bar_qfree[qb], ((units >> 1) - 1) & 1u, &s_abort, p.err) : !s_abort;
+      const bool go = units >= 2 ? q8_wait(&bar_qfree[qb], ((units >> 1) - 1) & 1u, &s_abort, p.err) : !s_abort;
       if (go) {
-        const UnitCols uc(p, S, qg, NQP);
+        const UnitCols<PAIR, NQP> uc(p, S, qg);
         unsigned char* qd = qs + qb * C::Q_BYTES;
         float* cd = cscale + (units & 3u) * NQP;
         constexpr int QB = NA < 8 ? NA : 8;  // vectors loaded at once
@@ -472,7 +612,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
             raw[i] = make_uint2(0, 0);
             if (n < uc.nvec) {
               const int e = uc.head(n), v = uc.vec(n);
-              if (p.pair) {
+              if (PAIR) {
                 if ((lane >> 4) == e)
                   raw[i] = *reinterpret_cast<const uint2*>(
                       q + ((long long)(S.q_row0 + v / p.G) * p.Hq + (2 * h + e) * p.G + v % p.G) * 64 + (lane & 15) * 4);
@@ -494,8 +634,8 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
             const int e = max(-100, q8_exponent(amax));
             const float sc = exp2_int(-e);
             uint32_t a1, a2, b1, b2;
-            q8_split(f[0] * sc, f[1] * sc, a1, a2);
-            q8_split(f[2] * sc, f[3] * sc, b1, b2);
+            q8_split(pk2(f[0] * sc, f[1] * sc), a1, a2);
+            q8_split(pk2(f[2] * sc, f[3] * sc), b1, b2);
             const uint32_t off = (uint32_t)((((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4);
             *reinterpret_cast<uint32_t*>(qd + n * 128 + off) = a1 | (b1 << 16);
             *reinterpret_cast<uint32_t*>(qd + (NQP + n) * 128 + off) = a2 | (b2 << 16);
@@ -512,24 +652,83 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
     }
     // the MMA warp's last commits land on these barriers before the CTA exits
     for (uint32_t k = (units > 2 ? units - 2 : 0); k < units; ++k)
-      tc_wait(&bar_qfree[k & 1u], (k >> 1) & 1u, &s_abort, p.err);
+      q8_wait(&bar_qfree[k & 1u], (k >> 1) & 1u, &s_abort, p.err);
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ exponents
+    // Word of a key: e_k, e_v of the (first) head, then of the pair's second head.
+    // Loaded past L1 (the append may write neighbouring bytes), a tile pair ahead
+    // of being stored; lane l takes keys l, l + 32, ...
+    UnitIter itr = make_iter();
+    uint32_t tt = 0;
+    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
+      const int h = u % p.Hkv;
+      const int n_t = (r_hi - r_lo + 2 * kTcTile - 1) / (2 * kTcTile);
+      const long long base = S.k_row0 * p.c.Hkv + (long long)(PAIR ? 2 * h : h) * p.c.max_seq;
+      const signed char* kp = reinterpret_cast<const signed char*>(p.c.ke) + base;
+      const signed char* vp = reinterpret_cast<const signed char*>(p.c.ve) + base;
+      uint32_t w[8];
+      auto load = [&](int t, uint32_t(&o)[8]) {
+        need_rows(itr, min(r_hi, r_lo + (t + 1) * 2 * kTcTile));
+        // all loads in flight at once: a key past the range reads the last one's
+        int e[4][8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = min(r_lo + t * 2 * kTcTile + i * 32 + lane, r_hi - 1);
+          e[0][i] = __ldcg(kp + key);
+          e[1][i] = __ldcg(vp + key);
+        }
+        if (PAIR) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = p.c.max_seq + min(r_lo + t * 2 * kTcTile + i * 32 + lane, r_hi - 1);
+            e[2][i] = __ldcg(kp + key);
+            e[3][i] = __ldcg(vp + key);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          o[i] = (uint32_t)(e[0][i] & 255) | (uint32_t)(e[1][i] & 255) << 8 | (uint32_t)(e[2][i] & 255) << 16 |
+                 (uint32_t)e[3][i] << 24;
+      };
+      load(0, w);
+      for (int t = 0; t < n_t; ++t, ++tt) {
+        uint32_t nx[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (t + 1 < n_t) load(t + 1, nx);
+        const int slot = (int)(tt % C::EXP_RING);
+        if (tt >= (uint32_t)C::EXP_RING) q8_wait(&bar_efree[slot], ((tt / C::EXP_RING) - 1) & 1u, &s_abort, p.err);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          exps[slot * 2 * kTcTile + i * 32 + lane] = w[i];
+          w[i] = nx[i];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_efull[slot]);
+      }
+    }
   } else {
     // ------------------------------------------------------------ softmax warps
-    const int sw = warp - 3;
+    const int sw = warp - 4;
+    const int g = sw / (4 * H);         // group: pairs i with i % G == g
     const int sq = sw & 3;              // warp within its column slice
-    const int col0 = (sw >> 2) * NL;    // first query column of this thread
+    const int col0 = ((sw >> 2) % H) * NL;  // first query column of this thread
     const int qd = warp & 3;            // TMEM lane quadrant this warp may access
-    const int stid = tid - 96;
+    const int stid = tid - 128 - g * SMT;  // thread within the group
     const int my_row = qd * 32 + lane;  // key of either tile, then head dim, this thread owns
     const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
+    unsigned char* pg = ps + g * C::P_BYTES;
+    int* rp = s_rp[g];
+    auto group_bar = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(SMT) : "memory"); };
+    auto all_bar = [&]() { asm volatile("bar.sync %0, %1;" ::"n"(1 + G), "n"(G * SMT) : "memory"); };
     UnitIter itr = make_iter();
-    uint32_t it = 0, tt = 0, pv = 0, units = 0;
+    uint32_t it = 0, units = 0;  // it: tile pairs before this unit
+    constexpr int NP = NL / 2;   // columns are worked on two at a time
+    const f32x2 c16 = pk2(0.0625f, 0.0625f);
     // columns past the unit's vectors hold anything: an MMA column enters no other
     while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
       const int h = u % p.Hkv, qg = u / p.Hkv;
       const int n_sub = (r_hi - r_lo + kTcTile - 1) / kTcTile;
       const int n_t = (n_sub + 1) >> 1;
-      const UnitCols uc(p, S, qg, NQP);
+      const UnitCols<PAIR, NQP> uc(p, S, qg);
       const int nvec = uc.nvec;
       if (nvec > NA && stid == 0) set_error(p.err, kErrBadRows);  // an item longer than the call's max_q
       const int c_first = (int)(ustart / share);
@@ -539,212 +738,247 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
       // (the plan kernel clears the counters, so they are read after it only)
       if (n_contrib > 1 && stid == 0 && itr.waited) arrived = ld_relaxed_gpu(p.ws_cnt + c_first);
 
-      // exponents of this thread's two keys (head pairs: of both heads), one tile
-      // pair ahead; loaded past L1, since the append may write neighbouring bytes
-      const long long ebase = S.k_row0 * p.c.Hkv + (long long)(p.pair ? 2 * h : h) * p.c.max_seq;
-      const int estep = p.pair ? p.c.max_seq : 0;
-      int ke[2][2], ve[2][2];  // [half][head of the pair]
-      auto load_exps = [&](int t) {
-        need_rows(itr, min(r_hi, r_lo + (t + 1) * 2 * kTcTile));
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int key = r_lo + (2 * t + hf) * kTcTile + my_row;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            ke[hf][e] = ve[hf][e] = 0;
-            if (key < r_hi) {
-              ke[hf][e] = __ldcg(reinterpret_cast<const signed char*>(p.c.ke) + ebase + e * estep + key);
-              ve[hf][e] = __ldcg(reinterpret_cast<const signed char*>(p.c.ve) + ebase + e * estep + key);
-            }
-          }
-        }
-      };
-      load_exps(0);
       if (p.row_pos != nullptr) {
         if (sq == 0 && lane < NL) {
           const int n = col0 + lane;
-          s_rp[n] = n < nvec ? p.row_pos[(long long)(S.q_row0 + uc.vec(n) / p.G) * p.row_pos_stride] : -1;
+          rp[n] = n < nvec ? p.row_pos[(long long)(S.q_row0 + uc.vec(n) / p.G) * p.row_pos_stride] : -1;
         }
-        softmax_bar<SMT>();
+        group_bar();
       }
-      tc_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
-      float csc[NL], m[NL], lp[NL], oacc[NL];
+      q8_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
+      const float* csc = cscale + (units & 3u) * NQP + col0;
+      // The running maximum of column col0 + j (j < NL) lives in lane j of every
+      // softmax warp of the slice: what the exponentials subtract (8 below it) and the
+      // pair's rescale factors reach the other lanes through shared memory.
+      float m = NEG_INF;
+      f32x2 lp[NP], oacc[NP];
 #pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        csc[j] = cscale[(units & 3u) * NQP + col0 + j];
-        m[j] = NEG_INF;
-        lp[j] = 0.f;
-        oacc[j] = 0.f;
-      }
-      auto add_o = [&]() {  // the last tile pair's P.V joins O
-        tc_wait(&bar_ofull, pv & 1u, &s_abort, p.err);
+      for (int j = 0; j < NP; ++j) lp[j] = oacc[j] = 0ull;
+      auto add_o = [&](uint32_t i) {  // P.V of pair i joins O
+        q8_wait(&bar_ofull[g], (i / G) & 1u, &s_abort, p.err);
         tc_fence_after();
-        float o0[NL], o1[NL], o2[NL], o3[NL];
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + col0), o0);
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + NQP + col0), o1);
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + N + col0), o2);
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + N + NQP + col0), o3);
+        float o0[NL], o1[NL];
+        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + g * N + col0), o0);
+        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + g * N + NQP + col0), o1);
         tc_wait_ld();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_ofree);
-        ++pv;
 #pragma unroll
-        for (int j = 0; j < NL; ++j) oacc[j] += fmaf(o1[j] + o3[j], 0.0625f, o0[j] + o2[j]);
+        for (int j = 0; j < NP; ++j)
+          oacc[j] = add2(oacc[j], fma2(pk2(o1[2 * j], o1[2 * j + 1]), c16, pk2(o0[2 * j], o0[2 * j + 1])));
       };
-      for (int t = 0; t < n_t; ++t) {
-        const uint32_t ti = tt + t;
-        const int sb = (int)(ti & 1u);
+      // a per-head pair of values for the columns (2 j, 2 j + 1)
+      auto by_head = [&](int j, float v0, float v1) {
+        if constexpr (!PAIR) return pk2(v0, v0);
+        return pk2(uc.head(col0 + 2 * j) ? v1 : v0, uc.head(col0 + 2 * j + 1) ? v1 : v0);
+      };
+      const int t0 = G == 1 ? 0 : (int)((it ^ (uint32_t)g) & 1u);  // this group's first pair
+      for (int t = t0; t < n_t; t += G) {
+        const uint32_t i = it + t;
+        const int sb = (int)(i & 1u);
         const int k0 = r_lo + t * 2 * kTcTile;
-        float ksc[2][2], vex[2][2];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            ksc[hf][e] = exp2_int(ke[hf][e]);
-            vex[hf][e] = (float)ve[hf][e];
-          }
-        if (t + 1 < n_t) load_exps(t + 1);
-        tc_wait(&bar_sfull[sb], (ti >> 1) & 1u, &s_abort, p.err);
+        const int es = (int)(i % C::EXP_RING);
+        q8_wait(&bar_efull[es], (i / C::EXP_RING) & 1u, &s_abort, p.err);
+        const uint32_t ew[2] = {exps[es * 2 * kTcTile + my_row], exps[es * 2 * kTcTile + kTcTile + my_row]};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_efree[es]);
+        q8_wait(&bar_sfull[sb], (i >> 1) & 1u, &s_abort, p.err);
         tc_fence_after();
-        float x[2][NL];
+        f32x2 x[2][NP];
         {
-          float lo[2][NL];
+          float hi[2][NL], lo[2][NL];
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            tmem_cols<NL>(tq + (uint32_t)((2 * sb + hf) * N + col0), x[hf]);
+            tmem_cols<NL>(tq + (uint32_t)((2 * sb + hf) * N + col0), hi[hf]);
             tmem_cols<NL>(tq + (uint32_t)((2 * sb + hf) * N + NQP + col0), lo[hf]);
           }
           tc_wait_ld();
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float ka = exp2_int((int)(signed char)ew[hf]), kb = exp2_int((int)(signed char)(ew[hf] >> 16));
+            const float va = (float)(signed char)(ew[hf] >> 8), vb = (float)(signed char)(ew[hf] >> 24);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+              const f32x2 s = fma2(pk2(lo[hf][2 * j], lo[hf][2 * j + 1]), c16, pk2(hi[hf][2 * j], hi[hf][2 * j + 1]));
+              const float2 cs = *reinterpret_cast<const float2*>(csc + 2 * j);
+              x[hf][j] = fma2(mul2(s, by_head(j, ka, kb)), pk2(cs.x, cs.y), by_head(j, va, vb));
+            }
+          }
+          // (after the scales are read: the Q warp may rewrite them once S is free)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_sfree[sb]);
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int j = 0; j < NL; ++j) {
-              const int e = uc.head(col0 + j);
-              x[hf][j] = fmaf(fmaf(lo[hf][j], 0.0625f, x[hf][j]) * ksc[hf][e], csc[j], vex[hf][e]);
-            }
         }
         // masking, as K2: nothing to do on a tile pair inside the unit and below the
         // causal frontier of the window's first row
-        const int tile_last = k0 + 2 * kTcTile - 1;
-        const bool interior = tile_last < r_hi && col0 + NL <= nvec && p.row_pos == nullptr &&
-                              tile_last <= S.k_len - S.q_len;
-        if (!interior) {
+        const int pair_last = k0 + 2 * kTcTile - 1;
+        if (pair_last >= r_hi || col0 + NL > nvec || p.row_pos != nullptr || pair_last > S.k_len - S.q_len) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             const int key = k0 + hf * kTcTile + my_row;
             const int nlim = key < r_hi ? nvec : 0;
             const int thr = (key - (S.k_len - S.q_len)) * p.G;
 #pragma unroll
-            for (int j = 0; j < NL; ++j) {
-              const int n = col0 + j;
-              const bool see = n < nlim && (p.row_pos != nullptr ? key <= s_rp[n] : uc.vec(n) >= thr);
-              x[hf][j] = see ? x[hf][j] : NEG_INF;
+            for (int j = 0; j < NP; ++j) {
+              float y[2];
+              up2(x[hf][j], y[0], y[1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int n = col0 + 2 * j + e;
+                const bool see = n < nlim && (p.row_pos != nullptr ? key <= rp[n] : uc.vec(n) >= thr);
+                y[e] = see ? y[e] : NEG_INF;
+              }
+              x[hf][j] = pk2(y[0], y[1]);
             }
           }
         }
-        float* rb = red + (ti & 1u) * (4 * NQP);
-        {
-          float r[NL];
+        float* rb = red + (2 * g + ((i / G) & 1u)) * (4 * NQP);
 #pragma unroll
-          for (int j = 0; j < NL; ++j) r[j] = warp_max_f32(fmaxf(x[0][j], x[1][j]));
-          if (lane == 0) {
-#pragma unroll
-            for (int j = 0; j < NL; ++j) rb[sq * NQP + col0 + j] = r[j];
-          }
+        for (int j = 0; j < NP; ++j) {
+          float a0, a1, b0, b1;
+          up2(x[0][j], a0, a1);
+          up2(x[1][j], b0, b1);
+          const float r0 = warp_max_f32(fmaxf(a0, b0)), r1 = warp_max_f32(fmaxf(a1, b1));
+          if (lane == 0) *reinterpret_cast<float2*>(rb + sq * NQP + col0 + 2 * j) = make_float2(r0, r1);
         }
-        softmax_bar<SMT>();
-        if (t >= 1) add_o();  // relative to the maximum before this tile; also frees P^T
-        // every thread keeps the running maxima of its columns
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int c = col0 + j;
+        group_bar();
+        if (t >= G) add_o(i - G);  // relative to the maximum before this pair; also frees P^T
+        float* mw = mxs + sw * 32;
+        float al = 1.f;
+        if (lane < NL) {
+          const int c = col0 + lane;
           const float mx = fmaxf(fmaxf(rb[c], rb[NQP + c]), fmaxf(rb[2 * NQP + c], rb[3 * NQP + c]));
-          if (mx > m[j] + 0.75f) {
-            const float al = fast_exp2(m[j] - mx);
-            lp[j] *= al;
-            oacc[j] *= al;
-            m[j] = mx;
+          if (mx > m + 0.75f) {
+            al = ex2_ftz(m - mx);
+            m = mx;
+          }
+          mw[lane] = m == NEG_INF ? 0.f : 8.f - m;  // no key seen: exp2(-inf) = 0
+          mw[16 + lane] = al;
+        }
+        const bool moved = __any_sync(0xffffffffu, al != 1.f);
+        __syncwarp();
+        if (moved) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const float2 aj = *reinterpret_cast<const float2*>(mw + 16 + 2 * j);
+            lp[j] = mul2(lp[j], pk2(aj.x, aj.y));
+            oacc[j] = mul2(oacc[j], pk2(aj.x, aj.y));
           }
         }
-        const int n_here = (2 * t + 1 < n_sub) ? 2 : 1;
+        if (pair_last >= r_hi && col0 == 0) {  // warp-uniform
+          // rows past the range may hold anything: once the pair has landed, zero these keys' V rows
+          q8_wait(&bar_vfull[i % VS], (i / VS) & 1u, &s_abort, p.err);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (hf < n_here) {
-            const int key = k0 + hf * kTcTile + my_row;
-            if (key >= r_hi && col0 == 0) {
-              // rows past the range may hold anything: zero this key's V row
-              unsigned char* vrow = kvs + (int)((it + 2 * t + hf) % STAGES) * C::KV_STAGE + C::TILE_BYTES + my_row * 128;
+          for (int hf = 0; hf < 2; ++hf) {
+            if (k0 + hf * kTcTile + my_row >= r_hi) {
+              unsigned char* vrow = vts + (int)(i % VS) * C::PAIR_BYTES + (hf * kTcTile + my_row) * 128;
 #pragma unroll
               for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vrow + c * 16) = make_uint4(0, 0, 0, 0);
             }
-            const float iv0 = exp2_int(-(int)vex[hf][0]), iv1 = exp2_int(-(int)vex[hf][1]);
-            uint32_t w1[(NL + 3) / 4], w2[(NL + 3) / 4];
-#pragma unroll
-            for (int j = 0; j < NL; j += 2) {
-              float w[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float mb = m[j + e] == NEG_INF ? 0.f : m[j + e] - 8.f;  // no key seen: exp2(-inf) = 0
-                w[e] = fast_exp2(x[hf][j + e] - mb);
-                lp[j + e] = fmaf(w[e], uc.head(col0 + j + e) ? iv1 : iv0, lp[j + e]);
-              }
-              uint32_t p1, p2;
-              q8_split(w[0], w[1], p1, p2);
-              if ((j & 2) == 0) {
-                w1[j / 4] = p1;
-                w2[j / 4] = p2;
-              } else {
-                w1[j / 4] |= p1 << 16;
-                w2[j / 4] |= p2 << 16;
-              }
-            }
-            const uint32_t rowo = (uint32_t)((hf * kTcTile + my_row) * C::P_ROWB);
-            auto put = [&](int col, const uint32_t(&w)[(NL + 3) / 4]) {
-              uint32_t off = rowo + (uint32_t)col;
-              off ^= ((off >> 7) & ((1u << C::P_SWZ_BITS) - 1u)) << 4;
-              if constexpr (NL == 16)
-                *reinterpret_cast<uint4*>(ps + off) = make_uint4(w[0], w[1], w[2], w[3]);
-              else if constexpr (NL == 8)
-                *reinterpret_cast<uint2*>(ps + off) = make_uint2(w[0], w[1]);
-              else if constexpr (NL == 4)
-                *reinterpret_cast<uint32_t*>(ps + off) = w[0];
-              else
-                *reinterpret_cast<uint16_t*>(ps + off) = (uint16_t)w[0];
-            };
-            put(col0, w1);
-            put(NQP + col0, w2);
           }
         }
+        // weights 2^(t - M + 8); the denominator's leave the value scale out again.
+        // (A pair of one tile: the other's are zero, and no MMA reads them.)
+        uint32_t w1[2][(NL + 3) / 4], w2[2][(NL + 3) / 4];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const float2 mj = *reinterpret_cast<const float2*>(mw + 2 * j);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float ia = exp2_int(-(int)(signed char)(ew[hf] >> 8)), ib = exp2_int(-(int)(signed char)(ew[hf] >> 24));
+            float d0, d1;
+            up2(add2(x[hf][j], pk2(mj.x, mj.y)), d0, d1);
+            const f32x2 w = pk2(ex2_ftz(d0), ex2_ftz(d1));
+            lp[j] = fma2(w, by_head(j, ia, ib), lp[j]);
+            uint32_t p1, p2;
+            q8_split(w, p1, p2);
+            if ((j & 1) == 0) {
+              w1[hf][j / 2] = p1;
+              w2[hf][j / 2] = p2;
+            } else {
+              w1[hf][j / 2] |= p1 << 16;
+              w2[hf][j / 2] |= p2 << 16;
+            }
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint32_t rowo = (uint32_t)((hf * kTcTile + my_row) * C::P_ROWB);
+          auto put = [&](int col, const uint32_t(&w)[(NL + 3) / 4]) {
+            uint32_t off = rowo + (uint32_t)col;
+            off ^= ((off >> 7) & ((1u << C::P_SWZ_BITS) - 1u)) << 4;
+            if constexpr (NL == 16)
+              *reinterpret_cast<uint4*>(pg + off) = make_uint4(w[0], w[1], w[2], w[3]);
+            else if constexpr (NL == 8)
+              *reinterpret_cast<uint2*>(pg + off) = make_uint2(w[0], w[1]);
+            else if constexpr (NL == 4)
+              *reinterpret_cast<uint32_t*>(pg + off) = w[0];
+            else
+              *reinterpret_cast<uint16_t*>(pg + off) = (uint16_t)w[0];
+          };
+          put(col0, w1[hf]);
+          put(NQP + col0, w2[hf]);
+        }
         fence_async_smem();
-        softmax_bar<SMT>();
-        if (stid == 0) mbar_arrive(&bar_pfull);
+        group_bar();
+        if (stid == 0) mbar_arrive(&bar_pfull[g]);
       }
-      add_o();
-      it += n_sub;
-      tt += n_t;
+      if (t0 < n_t) add_o(it + (uint32_t)(t0 + (n_t - 1 - t0) / G * G));
+      it += n_t;
       ++units;
 
       // ---- column sums of the weights over the unit's keys
-      float* lb = lred + (units & 1u) * (4 * NQP);
+      float* lb = lred + (2 * g + (units & 1u)) * (4 * NQP);
       {
         float w[NL];
 #pragma unroll
-        for (int j = 0; j < NL; ++j) w[j] = lp[j];
+        for (int j = 0; j < NP; ++j) up2(lp[j], w[2 * j], w[2 * j + 1]);
         const float r = warp_col_sum<NL>(w, lane);
         if (lane < NL) lb[sq * NQP + col0 + reduced_col<NL>(lane)] = r;
       }
-      softmax_bar<SMT>();
-      auto lsum = [&](int n) { return lb[n] + lb[NQP + n] + lb[2 * NQP + n] + lb[3 * NQP + n]; };
+      group_bar();
+      float mc[NL], lc[NL], oc[NL];
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int n = col0 + j;
+        mc[j] = __shfl_sync(0xffffffffu, m, j);
+        lc[j] = lb[n] + lb[NQP + n] + lb[2 * NQP + n] + lb[3 * NQP + n];
+      }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) up2(oacc[j], oc[2 * j], oc[2 * j + 1]);
+      if constexpr (G == 2) {
+        // the second group hands its (m, l, O) over through shared memory (O in its own
+        // P^T buffer, whose last P.V is done) and goes on to the next unit
+        float* og = reinterpret_cast<float*>(ps + C::P_BYTES);
+        if (g == 1) {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            og[j * kTcTile + my_row] = oc[j];
+            if (my_row == 0) {
+              ml[j] = mc[j];
+              ml[NQP + j] = lc[j];
+            }
+          }
+        }
+        all_bar();
+        if (g == 0) {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            const float m1 = ml[j], nm = fmaxf(mc[j], m1), ms = nm == NEG_INF ? 0.f : nm;
+            const float wa = ex2_ftz(mc[j] - ms), wb = ex2_ftz(m1 - ms);
+            lc[j] = lc[j] * wa + ml[NQP + j] * wb;
+            oc[j] = oc[j] * wa + og[j * kTcTile + my_row] * wb;
+            mc[j] = nm;
+          }
+        }
+        all_bar();
+        if (g == 1) continue;
+      }
       const int dim = my_row;
       // output element of query column n held by this thread's O^T row, or -1
       auto out_at = [&](int n) -> long long {
         const int e = uc.head(n), v = uc.vec(n);
         const long long row = (long long)(S.q_row0 + v / p.G) * p.Hq + v % p.G;
-        if (p.pair) return (dim >> 6) == e ? (row + (2 * h + e) * p.G) * 64 + (dim & 63) : -1;
+        if (PAIR) return (dim >> 6) == e ? (row + (2 * h + e) * p.G) * 64 + (dim & 63) : -1;
         return (row + h * p.G) * 128 + dim;
       };
       auto put_out = [&](int n, float O, float L) {
@@ -754,7 +988,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
       if (n_contrib == 1) {
 #pragma unroll
         for (int j = 0; j < NL; ++j)
-          if (col0 + j < nvec) put_out(col0 + j, oacc[j], lsum(col0 + j));
+          if (col0 + j < nvec) put_out(col0 + j, oc[j], lc[j]);
       } else {
         if (!itr.waited) {
           griddep_wait();
@@ -765,7 +999,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
           s_flag = (arrived == n_contrib - 1) ? 2 : 0;
           if (s_flag == 2) fence_acq_rel_gpu();
         }
-        softmax_bar<SMT>();
+        group_bar();
         if (s_flag != 2) {
           const int slot = (ustart < a) ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
           float* pb = p.ws_part + (size_t)slot * C::PART_FLOATS;
@@ -773,19 +1007,19 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
           for (int j = 0; j < NL; ++j) {
             if (col0 + j < nvec) {
               if (dim == 0) {
-                pb[col0 + j] = m[j];
-                pb[NQP + col0 + j] = lsum(col0 + j);
+                pb[col0 + j] = mc[j];
+                pb[NQP + col0 + j] = lc[j];
               }
-              pb[2 * NQP + (col0 + j) * 128 + dim] = oacc[j];
+              pb[2 * NQP + (col0 + j) * 128 + dim] = oc[j];
             }
           }
           __threadfence();
-          softmax_bar<SMT>();
+          group_bar();
           if (stid == 0) {
             const int prev = atomicAdd(p.ws_cnt + c_first, 1);
             s_flag = (prev == n_contrib - 1) ? 1 : 0;
           }
-          softmax_bar<SMT>();
+          group_bar();
         }
         if (s_flag) {
           __threadfence();
@@ -806,9 +1040,9 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
             for (int j = 0; j < NL; ++j) {
               const int n = col0 + j;
               if (k == k_own) {
-                mk[j] = m[j];
-                lk[j] = lsum(n);
-                ok[j] = oacc[j];
+                mk[j] = mc[j];
+                lk[j] = lc[j];
+                ok[j] = oc[j];
               } else {
                 mk[j] = n < nvec ? ld_cg_f32(base + n) : NEG_INF;
                 lk[j] = n < nvec ? ld_cg_f32(base + NQP + n) : 0.f;
@@ -830,7 +1064,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
             if (col0 + j < nvec) put_out(col0 + j, acc[j], Ls[j]);
         }
         if (s_flag && stid == 0) p.ws_cnt[c_first] = 0;
-        softmax_bar<SMT>();  // s_flag is rewritten by the next unit
+        group_bar();  // s_flag is rewritten by the next unit
       }
     }
   }
