@@ -315,6 +315,14 @@ def test_attn_many_items_shared_slots_and_offset(cuda_dev, kernel):
     run_attn(cuda_dev, n_slots=5, B=5, H=4, Hkv=2, Dh=128, S=70, items=items, kernel=kernel, slot_offset=2)
 
 
+@pytest.mark.parametrize("H,Hkv,Dh,q_len", [(8, 8, 64, 1), (16, 4, 128, 1), (16, 4, 128, 3), (16, 4, 128, 9)])
+def test_attn_long_streams(cuda_dev, H, Hkv, Dh, q_len):
+    """Enough work that every stream of every CTA goes round its rings several times and units straddle streams."""
+    n_slots, B = 4, 4
+    items = [(s, b, 5900 - 37 * b - 400 * s, q_len, (s * B + b) * q_len) for s in range(n_slots) for b in range(B)]
+    run_attn(cuda_dev, n_slots=n_slots, B=B, H=H, Hkv=Hkv, Dh=Dh, S=6000, items=items, kernel=1)
+
+
 def test_attn_two_items_on_one_position_store_the_later(cuda_dev):
     items = [(0, 0, 50, 4, 0), (0, 0, 52, 3, 4), (1, 0, 10, 1, 7), (1, 0, 10, 1, 8)]
     for kernel in (0, 1):

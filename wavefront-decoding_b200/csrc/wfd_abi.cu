@@ -1355,6 +1355,19 @@ int q8_cache(const wfd_q8_cache* c, int slot_offset, Q8Cache* out) {
   return WFD_OK;
 }
 
+// Scratch of one wfd_wave_attn_q8 call: up to two CTAs per SM.
+WsLayout q8_ws_layout(int n_items, int sms) {
+  WsLayout w;
+  const size_t shares = 2 * (size_t)sms;
+  w.cnt = 0;
+  w.part = align256(w.cnt + shares * sizeof(int));
+  w.segs = align256(w.part + 2 * shares * kVerifyMaxRows * (128 + 2) * sizeof(float));
+  w.prefix = align256(w.segs + (size_t)n_items * sizeof(Seg));
+  w.start = align256(w.prefix + (size_t)(n_items + 1) * sizeof(long long));
+  w.total = align256(w.start + shares * sizeof(CtaStart));
+  return w;
+}
+
 // (128 bytes, heads of 128 bytes, rows) view of a code buffer; box 128 bytes x 1 x
 // box_rows, 128-byte swizzle.
 bool make_q8_map(CUtensorMap* m, const void* base, long long rows, int row_bytes, int box_rows) {
@@ -1371,17 +1384,17 @@ bool make_q8_map(CUtensorMap* m, const void* base, long long rows, int row_bytes
 
 template <int NQP, int NA, bool PAIR>
 int launch_q8_tc(const Q8AttnParams& ap, const Q8Maps& maps, int sms, cudaStream_t st) {
-  using C = Q8Cfg<NQP, q8_groups(NA)>;
   static std::atomic<bool> attr_set[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WFD_ERR_CUDA;
   if (!attr_set[dev].load()) {
-    if (cudaFuncSetAttribute(q8_tc_kernel<NQP, NA, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(q8_tc_kernel<NQP, NA, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             q8_smem<NQP, NA>()) != cudaSuccess)
       return WFD_ERR_CUDA;
     attr_set[dev].store(true);
   }
-  return launch_pdl(q8_tc_kernel<NQP, NA, PAIR>, dim3(sms), dim3(q8_tc_threads(NA)), C::SMEM, st, maps, ap) ==
+  return launch_pdl(q8_tc_kernel<NQP, NA, PAIR>, dim3(q8_ctas(NA) * sms), dim3(q8_tc_threads(NA)), q8_smem<NQP, NA>(), st,
+                    maps, ap) ==
                  cudaSuccess
              ? WFD_OK
              : WFD_ERR_CUDA;
@@ -1509,7 +1522,7 @@ extern "C" int wfd_commit_window_q8(const wfd_q8_cache* cache, const wfd_item* i
 extern "C" size_t wfd_wave_attn_q8_workspace(int32_t n_items) {
   const int sms = current_sms();
   if (sms <= 0 || n_items < 0) return 0;
-  return ws_layout(n_items, 128, sms, true).total;
+  return q8_ws_layout(n_items, sms).total;
 }
 
 extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const void* q, const void* k_new,
@@ -1540,7 +1553,7 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   const bool tc_ok = dtype == WFD_DTYPE_BF16 && (c.Hkv * Dh) % 128 == 0 && key_rows < (1ll << 31);
   if (which < 0) which = tc_ok ? 1 : 0;
   if (which == 1 && !tc_ok) return WFD_ERR_UNSUPPORTED;
-  const WsLayout L = ws_layout(n_items, 128, sms, true);
+  const WsLayout L = q8_ws_layout(n_items, sms);
   if (workspace_bytes < L.total) return WFD_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
 
@@ -1575,7 +1588,7 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   pp.prefix = reinterpret_cast<long long*>(ws + L.prefix);
   if (!self_plan) {
     pp.start = reinterpret_cast<CtaStart*>(ws + L.start);
-    pp.seg_grid = sms;
+    pp.seg_grid = which == 1 && NQ == 16 ? 2 * sms : sms;
     pp.seg_units = tpair ? c.Hkv / 2 : c.Hkv;
   }
   pp.row_pos = row_pos;
@@ -1587,7 +1600,7 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   pp.lens_offset = slot_offset * c.n_seqs;
   pp.q8 = c;
   pp.zero = reinterpret_cast<int*>(ws + L.cnt);
-  pp.n_zero = sms;
+  pp.n_zero = 2 * sms;
   pp.min_share = kQ8MinShare;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 plan_grid(1 + (n_items < 4 * sms ? n_items : 4 * sms));

@@ -25,15 +25,21 @@
 // exceeds it by 3/4 (w <= 431 < 448).  The denominator needs 2^(s - M + 8) = w 2^{-e_v}.
 // |e_v| <= 32 keeps that above the fp32 underflow for every key that matters.
 //
-// What bounds it: HBM.  A tile pair (256 keys, 64 KB) takes 1.5 us of an SM's share
-// of the copy bandwidth; the softmax of a pair is one dependent chain through two
-// named barriers, so each softmax thread works on two keys (one of either tile):
-// the chain's latency is paid once per 64 KB, as in the bf16 kernel.
+// What bounds it: HBM; a step of 256 keys (64 KB of K and V) takes 1.5 us of an SM's
+// share of the copy bandwidth.  Behind it come two chains:
+//   * the softmax of a step is a dependent chain through two named barriers (1.5 us
+//     by itself).  Up to 16 query columns, two CTAs share an SM, each with a pipeline
+//     and a share of the work of its own, so that two chains, and the ends of units
+//     (output rows written or merged), overlap; a thread works on two keys, one of
+//     either tile, so that the chain is paid once per 64 KB.  32 columns need the
+//     registers of one CTA, whose 16 softmax warps are bound by instruction issue;
+//   * TMA keeps about 100 KB an SM in flight: 192 KB measured 12 % less bandwidth, and
+//     tensor maps that promote to 256 bytes fetch the neighbouring head's half of each
+//     pair of lines for nothing (53 % more DRAM traffic).
 //
-// Warp roles (one CTA per SM): 0 TMA producer; 1 TMEM owner and MMA issuer; 2 the
-// Q operand of the next units (two buffers); 3 the keys' exponents (a ring of tile
-// pairs); 4.. softmax, 4 warps per slice of the query columns.  Work split, merging and the self-planned start are K2's
-// (UnitIter, CtaStart).  Every wait is bounded; no multicast, no cluster.
+// Warp roles: 0 TMA producer; 1 TMEM owner and MMA issuer; 2 the Q operand of the next
+// unit; 3 the keys' exponents; 4.. softmax.  Work split, merging and the self-planned
+// start are K2's.  Every wait is bounded; no multicast, no cluster.
 #pragma once
 
 #include "wfd_q8_attn.cuh"
@@ -48,45 +54,38 @@ struct Q8Maps {
   CUtensorMap v[kQ8Boxes];
 };
 
-template <int NQP, int G>
+// CTAs an SM holds, column slices of the softmax (4 warps each), threads of a CTA.
+__host__ __device__ constexpr int q8_ctas(int na) { return na <= 16 ? 2 : 1; }
+__host__ __device__ constexpr int q8_slices(int na) { return na <= 16 ? 1 : 4; }
+__host__ __device__ constexpr int q8_tc_threads(int na) { return 128 + 128 * q8_slices(na); }
+
+template <int NQP, int NA>
 struct Q8Cfg {
   static constexpr int N = 2 * NQP;                  // MMA columns: both pieces
-  // Rings of tile pairs (256 keys x 128 bytes).  A K pair is done with after S, a V
-  // pair only after the softmax and P.V, one pair later: twice the V pairs keep as
-  // many of either in flight.
-  static constexpr int KS = 2;
-  static constexpr int VS = NQP == 16 ? 4 : 3;
+  static constexpr int CTAS = q8_ctas(NA);
+  static constexpr int T = NA == 16 ? 1 : 2;         // 128-key tiles of a step (16 columns a thread: one, for registers)
   static constexpr int TILE_BYTES = kTcTile * 128;
-  static constexpr int PAIR_BYTES = 2 * TILE_BYTES;
-  static constexpr int Q_BYTES = N * 128;            // one of two buffers
+  static constexpr int STEP_BYTES = T * TILE_BYTES;  // K (or V) of a step
+  // Rings of steps.  A K step is done with after S (of which there are as many
+  // buffers), a V step only after the softmax and P.V.
+  static constexpr int KS = CTAS == 2 && T == 2 ? 1 : 2;
+  static constexpr int VS = CTAS == 2 && T == 2 ? 2 : T == 2 ? 3 : 4;
+  static constexpr int Q_BYTES = N * 128;
+  static constexpr int QB = CTAS == 2 ? 1 : 2;       // Q operand buffers
   static constexpr int P_ROWB = N;                   // one key's row of P^T
-  static constexpr int P_BYTES = 2 * kTcTile * P_ROWB;     // one group's
+  static constexpr int P_BYTES = T * kTcTile * P_ROWB;
   static constexpr int P_SWZ_BITS = NQP == 16 ? 1 : 2;     // 32- / 64-byte swizzle
   static constexpr uint64_t P_LAYOUT = NQP == 16 ? 6 : 4;
   static constexpr int P_ATOM = 8 * P_ROWB;
-  static constexpr int RED_FLOATS = G * 2 * 4 * NQP;
-  static constexpr int EXP_RING = 4;                 // tile pairs of key / value exponents, one 32-bit word a key
-  static constexpr int EXP_BYTES = EXP_RING * 2 * kTcTile * 4;
-  static constexpr int MX_FLOATS = (NQP == 16 ? 8 : 16) * 2 * 16;  // per softmax warp: running maxima and rescale factors
-  static constexpr int ML_FLOATS = 2 * NQP;          // the second group's maxima and sums at the end of a unit
-  static constexpr int SMEM = (KS + VS) * PAIR_BYTES + 2 * Q_BYTES + G * P_BYTES + EXP_BYTES +
-                              (2 * RED_FLOATS + 4 * NQP + MX_FLOATS + ML_FLOATS) * 4 + 1024;
-  static constexpr int S_COL = 0;                    // S^T of tile pair buffer sb, half hf: (2 sb + hf) N
-  static constexpr int O_COL = 4 * N;                // O^T of group g: O_COL + g N
-  static constexpr int TMEM_COLS = NQP == 16 ? 256 : 512;
+  static constexpr int RED_FLOATS = 2 * 4 * NQP;     // double-buffered, 4 warps a slice
+  static constexpr int WARPS = 4 * q8_slices(NA);    // softmax warps
+  static constexpr int ER = 2;                       // exponent ring, in steps
+  static constexpr int S_COL = 0;                    // S^T buffer s, tile hf: (T s + hf) N
+  static constexpr int O_COL = KS * T * N;           // O^T
+  static constexpr int TMEM_COLS = O_COL + N <= 128 ? 128 : O_COL + N <= 256 ? 256 : 512;
   static constexpr int PART_FLOATS = NQP * (128 + 2);
-  static_assert(O_COL + G * N <= TMEM_COLS, "TMEM columns");
-  static_assert(SMEM + 2048 <= 232448, "shared memory per CTA (dynamic + the kernel's static arrays)");
+  static_assert(CTAS * TMEM_COLS <= 512 && O_COL + N <= TMEM_COLS, "TMEM columns");
 };
-
-// Softmax warps: groups that take alternate tile pairs, each with its own maxima,
-// sums and O (merged at the end of a unit), and slices of the query columns inside
-// a group.  Up to 16 columns a pair's softmax is a chain of dependent steps, and two
-// groups keep two pairs in it; 32 columns are bound by instruction issue, and four
-// slices of 8 fill the schedulers with less state a thread.
-__host__ __device__ constexpr int q8_groups(int na) { return na <= 16 ? 2 : 1; }
-__host__ __device__ constexpr int q8_slices(int na) { return na <= 16 ? 1 : na / 8; }
-__host__ __device__ constexpr int q8_tc_threads(int na) { return 128 + 128 * q8_groups(na) * q8_slices(na); }
 
 // kind::f8f6f4, e4m3 x e4m3 -> f32, M = 128
 __host__ __device__ constexpr uint32_t q8_idesc(int n, bool a_mn_major, bool b_mn_major) {
@@ -197,17 +196,91 @@ __device__ __forceinline__ void q8_split(f32x2 w, uint32_t& p1, uint32_t& p2) {
   p2 = e4m3x2(a, b);
 }
 
-// A CTA's share of the work and where it starts, from the item table itself (K2's
-// self-planned start: the plan kernel may still be running).  Called by the whole CTA.
+// A CTA's walk over its share [pos, end) of the work: the pieces [r_lo, r_hi) of
+// units (segment, query group, kv head), in order, as UnitIter's; a unit that follows
+// in the same segment costs no division and no load.
+struct Q8Stream {
+  long long pos, end, base, nbase, ustart;
+  Seg S;
+  int seg, u, r_lo, r_hi;
+  int t, n;        // step of the piece, steps of the piece
+  uint32_t step, unit;  // steps and units so far (the current one not counted)
+  bool fresh;      // u not yet known in this segment
+  bool live;
+  bool waited;     // griddep_wait() executed by this thread
+
+  __device__ __forceinline__ long long seg_base(const VerifyParams& p, int i) const {
+    return i <= p.n_segs - 1 ? (long long)p.Hkv * p.prefix[i] : 0x7fffffffffffffffll;
+  }
+  __device__ __forceinline__ bool next_unit(const VerifyParams& p, int step_keys) {
+    for (;;) {
+      if (pos >= end) {
+        live = false;
+        return false;
+      }
+      if (pos >= nbase) {
+        if (!waited) {  // the segment table and prefix are the plan kernel's outputs
+          griddep_wait();
+          waited = true;
+        }
+        while (pos >= nbase) {
+          ++seg;
+          base = nbase;
+          nbase = seg_base(p, seg + 1);
+        }
+        S = p.segs[seg];
+        fresh = true;
+      }
+      if (fresh) {
+        u = pos == base ? 0 : (int)((pos - base) / S.k_len);
+        ustart = base + (long long)u * S.k_len;
+        fresh = false;
+      } else {
+        ++u;
+        ustart += S.k_len;
+      }
+      const long long uend = ustart + S.k_len;
+      if (p.invariant) {
+        const bool mine = ustart >= pos;  // else it began in the share before this one, which takes it whole
+        pos = uend;
+        if (!mine) continue;
+        r_lo = 0;
+        r_hi = S.k_len;
+      } else {
+        r_lo = (int)(pos - ustart);
+        r_hi = (int)((uend < end ? uend : end) - ustart);
+        pos = ustart + r_hi;
+      }
+      t = 0;
+      n = (r_hi - r_lo + step_keys - 1) / step_keys;
+      return true;
+    }
+  }
+  // to the next step; returns whether there is one
+  __device__ __forceinline__ bool advance(const VerifyParams& p, int step_keys) {
+    ++step;
+    if (++t < n) return true;
+    ++unit;
+    return next_unit(p, step_keys);
+  }
+};
+
+// Where the CTA's share starts: from the item table itself (K2's self-planned start:
+// the plan kernel may still be running).  Called by the whole CTA.
 struct SelfStart {
   long long wtot[32];
   Seg S0;
   long long base0, nbase0;
   int seg0, slot0, seq0, minpos;
 };
+__device__ __forceinline__ void share_of(long long total, long long& share, long long& a, long long& b) {
+  share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
+  a = min(total, (long long)blockIdx.x * share);
+  b = min(total, a + share);
+}
 template <int THREADS>
-__device__ __forceinline__ long long self_start(const VerifyParams& p, SelfStart& sh, long long& share, long long& a,
-                                                long long& b) {
+__device__ __forceinline__ void self_start(const VerifyParams& p, SelfStart& sh, long long& share, long long& a,
+                                           long long& b) {
   constexpr int IPT = (kSelfPlanMax + THREADS - 1) / THREADS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wfd_item my[IPT];
@@ -238,14 +311,7 @@ __device__ __forceinline__ long long self_start(const VerifyParams& p, SelfStart
     before += (k < warp) ? sh.wtot[k] : 0;
     all += sh.wtot[k];
   }
-  const long long total = (long long)p.Hkv * all;
-  share = 1;
-  a = b = 0;
-  if (total > 0) {
-    share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
-    a = (long long)blockIdx.x * share;
-    b = (a + share < total) ? a + share : total;
-  }
+  share_of((long long)p.Hkv * all, share, a, b);
   if (a < b) {  // the item that holds work index a, by the thread that holds the item
     long long pf = before + incl - tsum;
 #pragma unroll
@@ -271,7 +337,35 @@ __device__ __forceinline__ long long self_start(const VerifyParams& p, SelfStart
     if (mp != 0x7fffffff) atomicMin(&sh.minpos, mp);
   }
   __syncthreads();
-  return total;
+}
+
+// Shared memory besides the tiles.
+template <typename C, int NQP>
+struct Q8Shared {
+  uint32_t exps[C::ER][C::T * kTcTile];  // a step's exponents, one word a key
+  float red[2][4][NQP];                  // column maxima of each warp
+  float lred[2][4][NQP];                 // column sums
+  float cscale[4][NQP];                  // score scale of each column, per unit
+  float mx[C::WARPS][2][16];             // per softmax warp: what the exponentials subtract, rescale factors
+  uint64_t kfull[C::KS], vfull[C::VS], vempty[C::VS];
+  uint64_t sfull[C::KS], sfree[C::KS];   // S of a step complete (its K free), and read by the softmax
+  uint64_t pfull, ofull;                 // P written (so the O of the step before is read), P.V complete
+  uint64_t qready[4], qfree[C::QB];      // a unit's Q operand and column scales written, its S MMAs done
+  uint64_t efull[C::ER], efree[C::ER];   // a step's exponents written, and read by every softmax warp
+  uint64_t drain;
+  SelfStart start;
+  uint32_t tmem;
+  int vslot[C::ER];                      // where the step's V tiles are: slot, phase parity << 8
+  int rp[NQP];                           // gapped windows: each query column's row position
+  int abort;
+  int flag;
+};
+template <int NQP, int NA>
+constexpr int q8_smem() {
+  using C = Q8Cfg<NQP, NA>;
+  constexpr int bytes = (C::KS + C::VS) * C::STEP_BYTES + C::QB * C::Q_BYTES + C::P_BYTES + (int)sizeof(Q8Shared<C, NQP>);
+  static_assert(C::CTAS * (bytes + 1024) <= 233472 && bytes <= 232448, "shared memory of an SM");
+  return bytes;
 }
 
 // The query columns of one unit: up to NQP vectors of one kv head, or up to NQP / 2
@@ -291,86 +385,61 @@ struct UnitCols {
 
 // NA: query columns the softmax works on (every unit has at most NA vectors).
 template <int NQP, int NA, bool PAIR>
-__global__ void __launch_bounds__(q8_tc_threads(NA), 1)
+__global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
     q8_tc_kernel(const __grid_constant__ Q8Maps maps, const Q8AttnParams p) {
-  constexpr int G = q8_groups(NA);   // softmax groups
-  constexpr int H = q8_slices(NA);   // column slices of a group (4 warps each)
-  using C = Q8Cfg<NQP, G>;
-  constexpr int KS = C::KS, VS = C::VS;
-  constexpr int N = C::N;
+  using C = Q8Cfg<NQP, NA>;
+  constexpr int T = C::T, KS = C::KS, VS = C::VS, N = C::N, ER = C::ER, QB = C::QB;
+  constexpr int STEP = T * kTcTile;  // keys of a step
   constexpr int THREADS = q8_tc_threads(NA);
+  constexpr int H = q8_slices(NA);   // column slices (4 warps each)
   constexpr int NL = NA / H;         // query columns per softmax thread
-  constexpr int SMT = 128 * H;       // softmax threads of a group
-  static_assert(4 * G * H * 32 <= C::MX_FLOATS && (G == 1 || NL * kTcTile * 4 <= C::P_BYTES), "the merge of two groups");
+  constexpr int NP = NL / 2;         // ... worked on two at a time
+  constexpr int SMT = 128 * H;       // softmax threads
   static_assert(NL == 2 || NL == 4 || NL == 8 || NL == 16, "columns per softmax thread");
   static_assert(NA <= NQP, "active query columns");
-  static_assert(KS == 2, "the K ring shares S's barriers");
   const float NEG_INF = -__int_as_float(0x7f800000);
 
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* kts = smem;                                // KS K tile pairs
-  unsigned char* vts = kts + KS * C::PAIR_BYTES;            // VS V tile pairs
-  unsigned char* qs = vts + VS * C::PAIR_BYTES;             // 2 x Q operand (K-major, 128B swizzle)
-  unsigned char* ps = qs + 2 * C::Q_BYTES;                  // P^T operand of a tile pair (MN-major), per group
-  float* red = reinterpret_cast<float*>(ps + G * C::P_BYTES);  // [G][2][4][NQP] column maxima
-  float* lred = red + C::RED_FLOATS;                        // [G][2][4][NQP] column sums
-  float* ml = lred + C::RED_FLOATS;                         // [2][NQP] the second group's maxima and sums
-  float* cscale = ml + C::ML_FLOATS;                     // [4][NQP] score scale of each column, per unit
-  float* mxs = cscale + 4 * NQP;                            // [16][2][16] per softmax warp
-  uint32_t* exps = reinterpret_cast<uint32_t*>(mxs + C::MX_FLOATS);  // [EXP_RING][2][128] exponents of a key
-
-  __shared__ __align__(8) uint64_t bar_kfull[KS];
-  __shared__ __align__(8) uint64_t bar_vfull[VS];
-  __shared__ __align__(8) uint64_t bar_vempty[VS];
-  __shared__ __align__(8) uint64_t bar_sfull[2];
-  __shared__ __align__(8) uint64_t bar_sfree[2];
-  __shared__ __align__(8) uint64_t bar_pfull[G];
-  __shared__ __align__(8) uint64_t bar_ofull[G];
-  __shared__ __align__(8) uint64_t bar_qready[4];  // unit's Q and column scales written
-  __shared__ __align__(8) uint64_t bar_qfree[2];
-  __shared__ __align__(8) uint64_t bar_drain;
-  __shared__ __align__(8) uint64_t bar_efull[C::EXP_RING];   // a tile pair's exponents written
-  __shared__ __align__(8) uint64_t bar_efree[C::EXP_RING];   // ... and read by every softmax warp
-  __shared__ uint32_t s_tmem;
-  __shared__ int s_rp[G][NQP];  // gapped windows: each query column's row position
-  __shared__ volatile int s_abort;
-  __shared__ int s_flag;
-  __shared__ SelfStart s_start;
+  extern __shared__ __align__(1024) unsigned char q8_raw[];
+  unsigned char* kts = q8_raw;                               // KS steps of K
+  unsigned char* vts = kts + KS * C::STEP_BYTES;             // VS steps of V
+  unsigned char* qs = vts + VS * C::STEP_BYTES;              // QB x Q operand (K-major, 128B swizzle)
+  unsigned char* ps = qs + QB * C::Q_BYTES;                  // P^T operand of a step (MN-major)
+  Q8Shared<C, NQP>& sh = *reinterpret_cast<Q8Shared<C, NQP>*>(ps + C::P_BYTES);
+  volatile int* abort_flag = &sh.abort;
+  // the swizzled tiles rely on the declared alignment (no room is kept to make up for it)
+  if ((smem_u32(q8_raw) & 1023u) != 0) {
+    set_error(p.err, kErrTimeout);
+    return;
+  }
 
   const int tid = threadIdx.x, warp = (int)uniform((uint32_t)tid >> 5), lane = tid & 31;
   const bool self = p.items != nullptr;
   if (tid == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k[0])) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v[0])) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.k[2 - T])) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.v[2 - T])) : "memory");
     for (int s = 0; s < KS; ++s) {
-      mbar_init(&bar_kfull[s], 1);
+      mbar_init(&sh.kfull[s], 1);
+      mbar_init(&sh.sfull[s], 1);
+      mbar_init(&sh.sfree[s], 4 * H);
     }
     for (int s = 0; s < VS; ++s) {
-      mbar_init(&bar_vfull[s], 1);
-      mbar_init(&bar_vempty[s], 1);
+      mbar_init(&sh.vfull[s], 1);
+      mbar_init(&sh.vempty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar_sfull[s], 1);
-      mbar_init(&bar_sfree[s], 4 * H);
-      mbar_init(&bar_qfree[s], 1);
+    mbar_init(&sh.pfull, 1);
+    mbar_init(&sh.ofull, 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&sh.qready[s], 1);
+    for (int s = 0; s < QB; ++s) mbar_init(&sh.qfree[s], 1);
+    for (int s = 0; s < ER; ++s) {
+      mbar_init(&sh.efull[s], 1);
+      mbar_init(&sh.efree[s], 4 * H);
     }
-    for (int s = 0; s < 4; ++s) mbar_init(&bar_qready[s], 1);
-    for (int s = 0; s < C::EXP_RING; ++s) {
-      mbar_init(&bar_efull[s], 1);
-      mbar_init(&bar_efree[s], 4 * H);
-    }
-    for (int s = 0; s < G; ++s) {
-      mbar_init(&bar_pfull[s], 1);
-      mbar_init(&bar_ofull[s], 1);
-    }
-    mbar_init(&bar_drain, 1);
+    mbar_init(&sh.drain, 1);
     fence_mbar_init();
-    s_abort = 0;
+    sh.abort = 0;
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                  "r"(C::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -379,251 +448,242 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = sh.tmem;
 
-  long long share = 1, a = 0, b = 0;
-  CtaStart cs{};
-  int minpos = 0;
-  if (self) {
-    self_start<THREADS>(p, s_start, share, a, b);
-    cs.S = s_start.S0;
-    cs.base = s_start.base0;
-    cs.nbase = s_start.nbase0;
-    cs.seg = s_start.seg0;
-    minpos = s_start.minpos;
-  } else {
-    cs = p.start[blockIdx.x];
-    const long long total = (long long)p.Hkv * p.prefix[p.n_segs];
-    if (total > 0) {
-      share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
-      a = (long long)blockIdx.x * share;
-      b = (a + share < total) ? a + share : total;
+  long long share, a, b;
+  if (self)
+    self_start<THREADS>(p, sh.start, share, a, b);
+  else
+    share_of((long long)p.Hkv * p.prefix[p.n_segs], share, a, b);
+  // every role walks the same steps
+  Q8Stream s;
+  s.pos = a;
+  s.end = b;
+  s.t = s.n = 0;
+  s.step = s.unit = 0;
+  s.fresh = true;
+  s.waited = !self;
+  s.live = a < b;
+  if (s.live) {
+    if (self) {
+      s.S = sh.start.S0;
+      s.base = sh.start.base0;
+      s.nbase = sh.start.nbase0;
+      s.seg = sh.start.seg0;
+    } else {
+      const CtaStart cs = p.start[blockIdx.x];
+      s.S = cs.S;
+      s.base = cs.base;
+      s.nbase = cs.nbase;
+      s.seg = cs.seg;
     }
+    s.next_unit(p, STEP);
   }
-  const int seg0 = cs.seg;
-  auto make_iter = [&]() {
-    UnitIter r{a, b, seg0};
-    if (a < b) {
-      r.have = true;
-      r.S = cs.S;
-      r.base = cs.base;
-      r.nbase = cs.nbase;
-    }
-    r.waited = !self;
-    return r;
-  };
-  // before reading cache rows (or their exponents) [.., end) of the current
+  // before reading cache rows (or their exponents) below `end` of the current
   // segment: the plan kernel's append may write rows from minpos on
-  auto need_rows = [&](UnitIter& itr, int end) {
-    if (!itr.waited && (itr.seg != seg0 || end > minpos)) {
+  auto need_rows = [&](int end) {
+    if (!s.waited && (s.seg != sh.start.seg0 || end > sh.start.minpos)) {
       griddep_wait();
-      itr.waited = true;
+      s.waited = true;
     }
   };
 
-  Seg S;
-  int u, r_lo, r_hi;
-  long long ustart;
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    UnitIter itr = make_iter();
-    uint32_t it = 0;
-    uint32_t n_k = 0, n_v = 0;  // pairs whose loads were issued (prefixes of the sequence: issue stops at an abort)
-    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
-      const int h = u % p.Hkv;
-      const int n_t = (r_hi - r_lo + 2 * kTcTile - 1) / (2 * kTcTile);
-      const long long row0 = S.k_row0 + p.k_row_offset + r_lo;
-      for (int t = 0; t < n_t; ++t, ++it) {
-        need_rows(itr, r_lo + (t + 1) * 2 * kTcTile);
-        const int row = (int)(row0 + (long long)t * 2 * kTcTile);
-        // a last pair of at most 224 keys loads only those, in boxes of 128 / 64 / 32 /
-        // 16 / 8 rows; what the stage holds past them is masked (V: zeroed)
-        const int left = r_hi - r_lo - t * 2 * kTcTile;
-        const int nr = left > 224 ? 2 * kTcTile : ((left + 7) & ~7);
-        auto load = [&](unsigned char* dst, const CUtensorMap* m, uint64_t* bar) {
-          mbar_arrive_expect_tx(bar, (uint32_t)(nr * 128));
-          if (nr == 2 * kTcTile) {
-            tma_load_3d(dst, m, 0, h, row, bar);
-          } else {
-            int off = 0;
-            for (int pc = 1; pc < kQ8Boxes; ++pc) {
-              const int pr = 256 >> pc;
-              if (nr & pr) {
-                tma_load_3d(dst + off * 128, m + pc, 0, h, row + off, bar);
-                off += pr;
-              }
+    uint32_t n_k = 0, n_v = 0;      // steps whose loads were issued (prefixes of the sequence: issue stops at an abort)
+    uint32_t ks = 0, vs = 0, kp = 0, vp = 0;  // ring slots and phases
+    while (s.live) {
+      need_rows(s.r_lo + (s.t + 1) * STEP);
+      const int h = s.u % p.Hkv;
+      const int row = (int)(s.S.k_row0 + p.k_row_offset + s.r_lo + (long long)s.t * STEP);
+      // a last step of few keys loads only those, in boxes of 128 / 64 / 32 / 16 / 8
+      // rows; what the stage holds past them is masked (V: zeroed)
+      const int left = s.r_hi - s.r_lo - s.t * STEP;
+      const int nr = left > STEP - 32 ? STEP : ((left + 7) & ~7);
+      auto load = [&](unsigned char* dst, const CUtensorMap* m, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, (uint32_t)(nr * 128));
+        if (nr == STEP) {
+          tma_load_3d(dst, m + (2 - T), 0, h, row, bar);
+        } else {
+          int off = 0;
+          for (int pc = 1; pc < kQ8Boxes; ++pc) {
+            const int pr = 256 >> pc;
+            if (nr & pr) {
+              tma_load_3d(dst + off * 128, m + pc, 0, h, row + off, bar);
+              off += pr;
             }
           }
-        };
-        const int ks = (int)(it % KS), vs = (int)(it % VS);
-        // (the K ring is as deep as S: pair it - 2's S complete frees its K)
-        bool go = it >= (uint32_t)KS ? q8_wait(&bar_sfull[ks], ((it / KS) - 1) & 1u, &s_abort, p.err) : !s_abort;
-        if (go && lane == 0) {
-          load(kts + ks * C::PAIR_BYTES, maps.k, &bar_kfull[ks]);
-          n_k = it + 1;
-          if (p.fail_waits && n_k == 1) {  // test hook: give up with this copy in flight
-            set_error(p.err, kErrTimeout);
-            s_abort = 1;
-          }
         }
-        __syncwarp();
-        go = it >= (uint32_t)VS ? q8_wait(&bar_vempty[vs], ((it / VS) - 1) & 1u, &s_abort, p.err) : !s_abort;
-        if (go && lane == 0) {
-          load(vts + vs * C::PAIR_BYTES, maps.v, &bar_vfull[vs]);
-          n_v = it + 1;
+      };
+      // (the K ring is as deep as S's: the S of step - KS complete frees its K)
+      bool go = s.step >= (uint32_t)KS ? q8_wait(&sh.sfull[ks], kp ^ 1u, abort_flag, p.err) : !*abort_flag;
+      go = __all_sync(0xffffffffu, go);
+      if (go && lane == 0) {
+        load(kts + ks * C::STEP_BYTES, maps.k, &sh.kfull[ks]);
+        n_k = s.step + 1;
+        if (p.fail_waits && n_k == 1) {  // test hook: give up with this copy in flight
+          set_error(p.err, kErrTimeout);
+          *abort_flag = 1;
         }
-        __syncwarp();
       }
+      __syncwarp();
+      go = s.step >= (uint32_t)VS ? q8_wait(&sh.vempty[vs], vp ^ 1u, abort_flag, p.err) : !*abort_flag;
+      go = __all_sync(0xffffffffu, go);
+      if (go && lane == 0) {
+        load(vts + vs * C::STEP_BYTES, maps.v, &sh.vfull[vs]);
+        n_v = s.step + 1;
+      }
+      __syncwarp();
+      if (++ks == KS) {
+        ks = 0;
+        kp ^= 1u;
+      }
+      if (++vs == VS) {
+        vs = 0;
+        vp ^= 1u;
+      }
+      s.advance(p, STEP);
     }
     // the MMA warp's commits land on these barriers before the CTA exits
-    for (uint32_t j = (it > (uint32_t)VS ? it - VS : 0); j < it; ++j)
-      q8_wait(&bar_vempty[j % VS], (j / VS) & 1u, &s_abort, p.err);
+    for (uint32_t j = (s.step > (uint32_t)VS ? s.step - VS : 0); j < s.step; ++j)
+      q8_wait(&sh.vempty[j % VS], (j / VS) & 1u, abort_flag, p.err);
     // copies in flight land before the CTA exits, also after an abort
     if (lane == 0) {
       for (uint32_t j = (n_k > (uint32_t)KS ? n_k - KS : 0); j < n_k; ++j)
-        if (!mbar_wait_bounded(&bar_kfull[j % KS], (j / KS) & 1u)) set_error(p.err, kErrTimeout);
+        if (!mbar_wait_bounded(&sh.kfull[j % KS], (j / KS) & 1u)) set_error(p.err, kErrTimeout);
       for (uint32_t j = (n_v > (uint32_t)VS ? n_v - VS : 0); j < n_v; ++j)
-        if (!mbar_wait_bounded(&bar_vfull[j % VS], (j / VS) & 1u)) set_error(p.err, kErrTimeout);
+        if (!mbar_wait_bounded(&sh.vfull[j % VS], (j / VS) & 1u)) set_error(p.err, kErrTimeout);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    UnitIter itr = make_iter();
-    uint32_t it = 0, units = 0;  // it: tile pairs before this unit
+    // S in order, ahead of the softmax; P.V as soon as a step's weights are there.
     constexpr uint32_t IDESC_S = q8_idesc(N, false, false);
     constexpr uint32_t IDESC_PV = q8_idesc(N, true, true);
-    const uint32_t q_addr = smem_u32(qs);
-    const uint32_t p_addr = smem_u32(ps);
-    const uint32_t k_addr = smem_u32(kts);
-    const uint32_t v_addr = smem_u32(vts);
+    const uint32_t q_addr = smem_u32(qs), p_addr = smem_u32(ps), k_addr = smem_u32(kts), v_addr = smem_u32(vts);
     const uint32_t tm = uniform(tmem);
-    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
-      const int n_sub = (r_hi - r_lo + kTcTile - 1) / kTcTile;
-      const int n_t = (n_sub + 1) >> 1;
-      const int qb = (int)(units & 1u);
-      const uint32_t qa = uniform(q_addr + (uint32_t)(qb * C::Q_BYTES));
-      q8_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
-      tc_fence_after();
-      // S of pair t + 1 goes out before P.V of pair t, whose weights the softmax is
-      // still computing; but when its keys are late, P.V does not wait for them
-      int ts = 0, tv = 0;
-      while (tv < n_t) {
-        bool do_s = ts < n_t, s_ok = false, p_ok = false;
-        if (do_s && tv < ts) {
-          const uint32_t i = it + ts, j = it + tv;
-          for (uint32_t n = 0; n < kSpinLimit; ++n) {  // (every exit by a vote)
-            s_ok = __all_sync(0xffffffffu, mbar_test_wait(&bar_kfull[i % KS], (i / KS) & 1u) &&
-                                               (i < 2 || mbar_test_wait(&bar_sfree[i & 1u], ((i >> 1) - 1) & 1u)));
-            if (s_ok) break;
-            p_ok = __all_sync(0xffffffffu, mbar_test_wait(&bar_pfull[j % G], (j / G) & 1u));
-            if (p_ok || __any_sync(0xffffffffu, s_abort != 0)) break;
-          }
-          do_s = !p_ok;
-        }
-        if (do_s) {
-          const uint32_t i = it + ts;
-          const int sb = (int)(i & 1u), ks = (int)(i % KS);
-          const bool two = uniform(2 * ts + 1 < n_sub) != 0;
-          bool go = s_ok;
-          if (!s_ok) {
-            go = q8_wait(&bar_kfull[ks], (i / KS) & 1u, &s_abort, p.err);
-            if (i >= 2) go = q8_wait(&bar_sfree[sb], ((i >> 1) - 1) & 1u, &s_abort, p.err) && go;
-          }
-          tc_fence_after();
-          const uint32_t k0 = uniform(k_addr + (uint32_t)(ks * C::PAIR_BYTES));
-          const uint32_t d0 = uniform(tm + (uint32_t)(2 * sb * N));
-          if (go && elect_lane()) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {  // 32 bytes of the row; the two tiles are independent accumulators
-              umma_f8(d0, umma_desc(k0 + j * 32, 16, 1024, 2), umma_desc(qa + j * 32, 16, 1024, 2), IDESC_S,
-                      j > 0 ? 1u : 0u);
-              if (two)
-                umma_f8(d0 + N, umma_desc(k0 + C::TILE_BYTES + j * 32, 16, 1024, 2),
-                        umma_desc(qa + j * 32, 16, 1024, 2), IDESC_S, j > 0 ? 1u : 0u);
-            }
-            umma_commit(&bar_sfull[sb]);
-            if (ts == n_t - 1) umma_commit(&bar_qfree[qb]);  // the unit's Q buffer may be rewritten
-          }
-          __syncwarp();
-          ++ts;
-        } else {
-          const uint32_t i = it + tv;
-          const int vs = (int)(i % VS);
-          const bool two = uniform(2 * tv + 1 < n_sub) != 0;
-          bool go = q8_wait(&bar_vfull[vs], (i / VS) & 1u, &s_abort, p.err);
-          const int g = (int)(i % G);
-          // (P of pair i written: the group has read S and the O of its pair before)
-          if (!p_ok) go = q8_wait(&bar_pfull[g], (i / G) & 1u, &s_abort, p.err) && go;
-          tc_fence_after();
-          const uint32_t v0 = uniform(v_addr + (uint32_t)(vs * C::PAIR_BYTES));
-          const uint32_t o0 = uniform(tm + (uint32_t)(C::O_COL + g * N));
-          const uint32_t p0 = uniform(p_addr + (uint32_t)(g * C::P_BYTES));
-          if (go && elect_lane()) {
-            // k-step j: 32 keys, four 8-row groups of V and of P^T
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
-                      umma_desc(p0 + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, j > 0 ? 1u : 0u);
-            if (two) {
-#pragma unroll
-              for (int j = 4; j < 8; ++j)
-                umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
-                        umma_desc(p0 + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, 1u);
-            }
-            umma_commit(&bar_ofull[g]);
-            umma_commit(&bar_vempty[vs]);
-          }
-          __syncwarp();
-          ++tv;
-        }
+    uint32_t ks = 0, vs = 0, kp = 0;   // of S's step
+    uint32_t pv = 0, pvs = 0, pvp = 0; // P.V issued so far, its V slot and phase
+    uint32_t two_tiles = 0;            // of the steps pv, pv + 1, ..: whether they have a second tile
+    // P.V of the next step, if its weights and its V tiles are there (last: waits)
+    auto try_pv = [&](uint32_t steps, bool last) -> bool {
+      if (pv == steps) return false;
+      bool go = __all_sync(0xffffffffu, mbar_test_wait(&sh.pfull, pv & 1u) && mbar_test_wait(&sh.vfull[pvs], pvp));
+      if (!go && !last) return false;
+      if (!go) {
+        go = q8_wait(&sh.pfull, pv & 1u, abort_flag, p.err);
+        go = q8_wait(&sh.vfull[pvs], pvp, abort_flag, p.err) && go;
       }
-      it += n_t;
-      ++units;
+      const bool two = uniform(two_tiles & 1u) != 0;
+      tc_fence_after();
+      const uint32_t v0 = uniform(v_addr + pvs * C::STEP_BYTES);
+      if (go && elect_lane()) {
+        const uint32_t o0 = tm + (uint32_t)C::O_COL;
+        // k-step j: 32 keys, four 8-row groups of V and of P^T
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
+                  umma_desc(p_addr + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, j > 0 ? 1u : 0u);
+        if (T == 2 && two) {
+#pragma unroll
+          for (int j = 4; j < 8; ++j)
+            umma_f8(o0, umma_desc(v0 + j * 4096, 16, 1024, 2),
+                    umma_desc(p_addr + j * 4 * C::P_ATOM, 16, C::P_ATOM, C::P_LAYOUT), IDESC_PV, 1u);
+        }
+        umma_commit(&sh.ofull);
+        umma_commit(&sh.vempty[pvs]);
+      }
+      __syncwarp();
+      two_tiles >>= 1;
+      ++pv;
+      if (++pvs == VS) {
+        pvs = 0;
+        pvp ^= 1u;
+      }
+      return true;
+    };
+    while (s.live) {
+      const uint32_t qpar = (s.unit >> 2) & 1u, spar = ((s.step / KS) & 1u) ^ 1u;
+      bool go = false;
+      for (uint32_t n = 0; n < kSpinLimit; ++n) {  // (every exit by a vote)
+        go = __all_sync(0xffffffffu, mbar_test_wait(&sh.kfull[ks], kp) &&
+                                         (s.step < (uint32_t)KS || mbar_test_wait(&sh.sfree[ks], spar)) &&
+                                         (s.t > 0 || mbar_test_wait(&sh.qready[s.unit & 3u], qpar)));
+        if (go) break;
+        if (!try_pv(s.step, false) && __any_sync(0xffffffffu, *abort_flag != 0)) break;
+      }
+      if (!go) q8_wait(&sh.kfull[ks], kp, abort_flag, p.err);  // an abort, or the spin limit
+      tc_fence_after();
+      const int left = s.r_hi - s.r_lo - s.t * STEP;
+      const bool two = uniform(left > kTcTile) != 0;
+      const uint32_t qb = s.unit % QB;
+      const uint32_t k0 = uniform(k_addr + ks * C::STEP_BYTES);
+      const uint32_t qa = uniform(q_addr + qb * C::Q_BYTES);
+      const uint32_t d0 = uniform(tm + ks * (uint32_t)(T * N));
+      if (go && elect_lane()) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // 32 bytes of the row; the tiles are independent accumulators
+          umma_f8(d0, umma_desc(k0 + j * 32, 16, 1024, 2), umma_desc(qa + j * 32, 16, 1024, 2), IDESC_S,
+                  j > 0 ? 1u : 0u);
+          if (T == 2 && two)
+            umma_f8(d0 + N, umma_desc(k0 + C::TILE_BYTES + j * 32, 16, 1024, 2), umma_desc(qa + j * 32, 16, 1024, 2),
+                    IDESC_S, j > 0 ? 1u : 0u);
+        }
+        umma_commit(&sh.sfull[ks]);
+        if (s.t == s.n - 1) umma_commit(&sh.qfree[qb]);  // the unit's Q buffer may be rewritten
+      }
+      __syncwarp();
+      two_tiles |= (two ? 1u : 0u) << (s.step - pv);
+      if (++ks == KS) {
+        ks = 0;
+        kp ^= 1u;
+      }
+      s.advance(p, STEP);
+    }
+    while (try_pv(s.step, true)) {
     }
     // every MMA complete before TMEM is freed and the CTA exits, also after an abort
     if (elect_lane()) {
-      umma_commit(&bar_drain);
-      if (!mbar_wait_bounded(&bar_drain, 0)) set_error(p.err, kErrTimeout);
+      umma_commit(&sh.drain);
+      if (!mbar_wait_bounded(&sh.drain, 0)) set_error(p.err, kErrTimeout);
     }
     __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------ Q operand
     // Lane l holds bytes 4l..4l+3 of a 128-byte row.  Rows n and NQP + n: the two
-    // pieces of query vector n.  The operand has two buffers (unit w is written once
-    // the S MMAs of unit w - 2 are done), its barriers and the column scales four:
-    // the softmax, two tile pairs behind the MMA warp, may still be in unit w - 3.
-    UnitIter itr = make_iter();
-    uint32_t units = 0;
+    // pieces of query vector n.  An operand buffer is rewritten once the S MMAs of its
+    // unit are done; the column scales and barriers have four turns, since the softmax
+    // may still be a unit behind the MMA warp.
     const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
-    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
-      const int h = u % p.Hkv, qg = u / p.Hkv;
-      const int qb = (int)(units & 1u);
-      const bool go = units >= 2 ? q8_wait(&bar_qfree[qb], ((units >> 1) - 1) & 1u, &s_abort, p.err) : !s_abort;
+    while (s.live) {
+      const int h = s.u % p.Hkv, qg = s.u / p.Hkv;
+      const uint32_t w = s.unit, qb = w % QB;
+      bool go = w >= (uint32_t)QB ? q8_wait(&sh.qfree[qb], ((w / QB) - 1) & 1u, abort_flag, p.err) : !*abort_flag;
+      go = __all_sync(0xffffffffu, go);
       if (go) {
-        const UnitCols<PAIR, NQP> uc(p, S, qg);
+        const UnitCols<PAIR, NQP> uc(p, s.S, qg);
         unsigned char* qd = qs + qb * C::Q_BYTES;
-        float* cd = cscale + (units & 3u) * NQP;
-        constexpr int QB = NA < 8 ? NA : 8;  // vectors loaded at once
-        for (int n0 = 0; n0 < NA; n0 += QB) {
-          uint2 raw[QB];
+        float* cd = sh.cscale[w & 3u];
+        constexpr int NB = NA < 8 ? NA : 8;  // vectors loaded at once
+        for (int n0 = 0; n0 < NA; n0 += NB) {
+          uint2 raw[NB];
 #pragma unroll
-          for (int i = 0; i < QB; ++i) {
+          for (int i = 0; i < NB; ++i) {
             const int n = n0 + i;
             raw[i] = make_uint2(0, 0);
             if (n < uc.nvec) {
               const int e = uc.head(n), v = uc.vec(n);
+              const long long row = (long long)(s.S.q_row0 + v / p.G) * p.Hq + v % p.G;
               if (PAIR) {
                 if ((lane >> 4) == e)
-                  raw[i] = *reinterpret_cast<const uint2*>(
-                      q + ((long long)(S.q_row0 + v / p.G) * p.Hq + (2 * h + e) * p.G + v % p.G) * 64 + (lane & 15) * 4);
+                  raw[i] = *reinterpret_cast<const uint2*>(q + (row + (2 * h + e) * p.G) * 64 + (lane & 15) * 4);
               } else {
-                raw[i] = *reinterpret_cast<const uint2*>(
-                    q + ((long long)(S.q_row0 + v / p.G) * p.Hq + h * p.G + v % p.G) * 128 + lane * 4);
+                raw[i] = *reinterpret_cast<const uint2*>(q + (row + h * p.G) * 128 + lane * 4);
               }
             }
           }
 #pragma unroll
-          for (int i = 0; i < QB; ++i) {
+          for (int i = 0; i < NB; ++i) {
             const int n = n0 + i;
             float f[4] = {__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xffff0000u),
                           __uint_as_float(raw[i].y << 16), __uint_as_float(raw[i].y & 0xffff0000u)};
@@ -647,119 +707,112 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
         fence_async_smem();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_qready[units & 3u]);
-      ++units;
+      if (lane == 0) mbar_arrive(&sh.qready[w & 3u]);
+      s.step += (uint32_t)s.n;
+      ++s.unit;
+      s.next_unit(p, STEP);
     }
     // the MMA warp's last commits land on these barriers before the CTA exits
-    for (uint32_t k = (units > 2 ? units - 2 : 0); k < units; ++k)
-      q8_wait(&bar_qfree[k & 1u], (k >> 1) & 1u, &s_abort, p.err);
+    for (uint32_t k = (s.unit > (uint32_t)QB ? s.unit - QB : 0); k < s.unit; ++k)
+      q8_wait(&sh.qfree[k % QB], (k / QB) & 1u, abort_flag, p.err);
   } else if (warp == 3) {
     // ------------------------------------------------------------ exponents
     // Word of a key: e_k, e_v of the (first) head, then of the pair's second head.
-    // Loaded past L1 (the append may write neighbouring bytes), a tile pair ahead
-    // of being stored; lane l takes keys l, l + 32, ...
-    UnitIter itr = make_iter();
-    uint32_t tt = 0;
-    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
-      const int h = u % p.Hkv;
-      const int n_t = (r_hi - r_lo + 2 * kTcTile - 1) / (2 * kTcTile);
-      const long long base = S.k_row0 * p.c.Hkv + (long long)(PAIR ? 2 * h : h) * p.c.max_seq;
+    // Loaded past L1 (the append may write neighbouring bytes), a step ahead of being
+    // stored; lane l takes keys l, l + 32, ...  A key past the range reads the last one's.
+    constexpr int NK = STEP / 32;
+    uint32_t w[NK];
+    uint32_t vs = 0, vp = 0, held = 0;  // V slot of the next step to load; of the step held in w
+    auto store = [&](uint32_t i) {      // step i, held in w
+      const int slot = (int)(i % ER);
+      if (i >= (uint32_t)ER) q8_wait(&sh.efree[slot], ((i / ER) - 1) & 1u, abort_flag, p.err);
+#pragma unroll
+      for (int k = 0; k < NK; ++k) sh.exps[slot][k * 32 + lane] = w[k];
+      if (lane == 0) sh.vslot[slot] = (int)held;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.efull[slot]);
+    };
+    while (s.live) {
+      const int h = s.u % p.Hkv;
+      const int k0 = s.r_lo + s.t * STEP;
+      need_rows(min(s.r_hi, k0 + STEP));
+      const long long base = s.S.k_row0 * p.c.Hkv + (long long)(PAIR ? 2 * h : h) * p.c.max_seq;
       const signed char* kp = reinterpret_cast<const signed char*>(p.c.ke) + base;
-      const signed char* vp = reinterpret_cast<const signed char*>(p.c.ve) + base;
-      uint32_t w[8];
-      auto load = [&](int t, uint32_t(&o)[8]) {
-        need_rows(itr, min(r_hi, r_lo + (t + 1) * 2 * kTcTile));
-        // all loads in flight at once: a key past the range reads the last one's
-        int e[4][8] = {};
+      const signed char* vq = reinterpret_cast<const signed char*>(p.c.ve) + base;
+      int e[4][NK] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = min(r_lo + t * 2 * kTcTile + i * 32 + lane, r_hi - 1);
-          e[0][i] = __ldcg(kp + key);
-          e[1][i] = __ldcg(vp + key);
-        }
+      for (int i = 0; i < NK; ++i) {
+        const int key = min(k0 + i * 32 + lane, s.r_hi - 1);
+        e[0][i] = __ldcg(kp + key);
+        e[1][i] = __ldcg(vq + key);
         if (PAIR) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = p.c.max_seq + min(r_lo + t * 2 * kTcTile + i * 32 + lane, r_hi - 1);
-            e[2][i] = __ldcg(kp + key);
-            e[3][i] = __ldcg(vp + key);
-          }
+          e[2][i] = __ldcg(kp + p.c.max_seq + key);
+          e[3][i] = __ldcg(vq + p.c.max_seq + key);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          o[i] = (uint32_t)(e[0][i] & 255) | (uint32_t)(e[1][i] & 255) << 8 | (uint32_t)(e[2][i] & 255) << 16 |
-                 (uint32_t)e[3][i] << 24;
-      };
-      load(0, w);
-      for (int t = 0; t < n_t; ++t, ++tt) {
-        uint32_t nx[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (t + 1 < n_t) load(t + 1, nx);
-        const int slot = (int)(tt % C::EXP_RING);
-        if (tt >= (uint32_t)C::EXP_RING) q8_wait(&bar_efree[slot], ((tt / C::EXP_RING) - 1) & 1u, &s_abort, p.err);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          exps[slot * 2 * kTcTile + i * 32 + lane] = w[i];
-          w[i] = nx[i];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_efull[slot]);
       }
+      if (s.step > 0) store(s.step - 1);
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        w[i] = (uint32_t)(e[0][i] & 255) | (uint32_t)(e[1][i] & 255) << 8 | (uint32_t)(e[2][i] & 255) << 16 |
+               (uint32_t)e[3][i] << 24;
+      held = vs | vp << 8;
+      if (++vs == VS) {
+        vs = 0;
+        vp ^= 1u;
+      }
+      s.advance(p, STEP);
     }
+    if (s.step > 0) store(s.step - 1);
   } else {
     // ------------------------------------------------------------ softmax warps
     const int sw = warp - 4;
-    const int g = sw / (4 * H);         // group: pairs i with i % G == g
-    const int sq = sw & 3;              // warp within its column slice
-    const int col0 = ((sw >> 2) % H) * NL;  // first query column of this thread
-    const int qd = warp & 3;            // TMEM lane quadrant this warp may access
-    const int stid = tid - 128 - g * SMT;  // thread within the group
-    const int my_row = qd * 32 + lane;  // key of either tile, then head dim, this thread owns
+    const int sq = sw & 3;                  // warp within its column slice
+    const int col0 = (sw >> 2) * NL;        // first query column of this thread
+    const int qd = warp & 3;                // TMEM lane quadrant this warp may access
+    const int stid = tid - 128;
+    const int my_row = qd * 32 + lane;      // key of a tile, then head dim, this thread owns
     const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
-    unsigned char* pg = ps + g * C::P_BYTES;
-    int* rp = s_rp[g];
-    auto group_bar = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(SMT) : "memory"); };
-    auto all_bar = [&]() { asm volatile("bar.sync %0, %1;" ::"n"(1 + G), "n"(G * SMT) : "memory"); };
-    UnitIter itr = make_iter();
-    uint32_t it = 0, units = 0;  // it: tile pairs before this unit
-    constexpr int NP = NL / 2;   // columns are worked on two at a time
+    const int vid = (int)blockIdx.x;
+    float* mw = sh.mx[sw][0];
     const f32x2 c16 = pk2(0.0625f, 0.0625f);
     // columns past the unit's vectors hold anything: an MMA column enters no other
-    while (itr.next(p, S, u, r_lo, r_hi, ustart)) {
-      const int h = u % p.Hkv, qg = u / p.Hkv;
-      const int n_sub = (r_hi - r_lo + kTcTile - 1) / kTcTile;
-      const int n_t = (n_sub + 1) >> 1;
+    while (s.live) {
+      const int h = s.u % p.Hkv, qg = s.u / p.Hkv;
+      const Seg S = s.S;
+      const int r_lo = s.r_lo, r_hi = s.r_hi, n_t = s.n;
+      const long long ustart = s.ustart;
       const UnitCols<PAIR, NQP> uc(p, S, qg);
       const int nvec = uc.nvec;
       if (nvec > NA && stid == 0) set_error(p.err, kErrBadRows);  // an item longer than the call's max_q
-      const int c_first = (int)(ustart / share);
-      const int c_last = (int)((ustart + S.k_len - 1) / share);
+      // the shares that hold keys of this unit
+      const int c_first = ustart >= a ? vid : (int)(ustart / share);
+      const int c_last = ustart + S.k_len <= a + share ? vid : (int)((ustart + S.k_len - 1) / share);
       const int n_contrib = p.invariant ? 1 : c_last - c_first + 1;
       int arrived = 0;
       // (the plan kernel clears the counters, so they are read after it only)
-      if (n_contrib > 1 && stid == 0 && itr.waited) arrived = ld_relaxed_gpu(p.ws_cnt + c_first);
-
+      if (n_contrib > 1 && stid == 0 && s.waited) arrived = ld_relaxed_gpu(p.ws_cnt + c_first);
       if (p.row_pos != nullptr) {
         if (sq == 0 && lane < NL) {
           const int n = col0 + lane;
-          rp[n] = n < nvec ? p.row_pos[(long long)(S.q_row0 + uc.vec(n) / p.G) * p.row_pos_stride] : -1;
+          sh.rp[n] = n < nvec ? p.row_pos[(long long)(S.q_row0 + uc.vec(n) / p.G) * p.row_pos_stride] : -1;
         }
-        group_bar();
+        softmax_bar<SMT>();
       }
-      q8_wait(&bar_qready[units & 3u], (units >> 2) & 1u, &s_abort, p.err);
-      const float* csc = cscale + (units & 3u) * NQP + col0;
+      q8_wait(&sh.qready[s.unit & 3u], (s.unit >> 2) & 1u, abort_flag, p.err);
+      const float* csc = sh.cscale[s.unit & 3u] + col0;
       // The running maximum of column col0 + j (j < NL) lives in lane j of every
       // softmax warp of the slice: what the exponentials subtract (8 below it) and the
-      // pair's rescale factors reach the other lanes through shared memory.
+      // step's rescale factors reach the other lanes through shared memory.
       float m = NEG_INF;
       f32x2 lp[NP], oacc[NP];
 #pragma unroll
       for (int j = 0; j < NP; ++j) lp[j] = oacc[j] = 0ull;
-      auto add_o = [&](uint32_t i) {  // P.V of pair i joins O
-        q8_wait(&bar_ofull[g], (i / G) & 1u, &s_abort, p.err);
+      auto add_o = [&](uint32_t i) {  // P.V of step i joins O
+        q8_wait(&sh.ofull, i & 1u, abort_flag, p.err);
         tc_fence_after();
         float o0[NL], o1[NL];
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + g * N + col0), o0);
-        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + g * N + NQP + col0), o1);
+        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + col0), o0);
+        tmem_cols<NL>(tq + (uint32_t)(C::O_COL + NQP + col0), o1);
         tc_wait_ld();
         tc_fence_before();
 #pragma unroll
@@ -771,49 +824,50 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
         if constexpr (!PAIR) return pk2(v0, v0);
         return pk2(uc.head(col0 + 2 * j) ? v1 : v0, uc.head(col0 + 2 * j + 1) ? v1 : v0);
       };
-      const int t0 = G == 1 ? 0 : (int)((it ^ (uint32_t)g) & 1u);  // this group's first pair
-      for (int t = t0; t < n_t; t += G) {
-        const uint32_t i = it + t;
-        const int sb = (int)(i & 1u);
-        const int k0 = r_lo + t * 2 * kTcTile;
-        const int es = (int)(i % C::EXP_RING);
-        q8_wait(&bar_efull[es], (i / C::EXP_RING) & 1u, &s_abort, p.err);
-        const uint32_t ew[2] = {exps[es * 2 * kTcTile + my_row], exps[es * 2 * kTcTile + kTcTile + my_row]};
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_efree[es]);
-        q8_wait(&bar_sfull[sb], (i >> 1) & 1u, &s_abort, p.err);
-        tc_fence_after();
-        f32x2 x[2][NP];
-        {
-          float hi[2][NL], lo[2][NL];
+      for (int t = 0; t < n_t; ++t) {
+        const uint32_t i = s.step + (uint32_t)t;
+        const int k0 = r_lo + t * STEP;
+        const int es = (int)(i % ER), sb = (int)(i % KS);
+        q8_wait(&sh.efull[es], (i / ER) & 1u, abort_flag, p.err);
+        uint32_t ew[T];
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            tmem_cols<NL>(tq + (uint32_t)((2 * sb + hf) * N + col0), hi[hf]);
-            tmem_cols<NL>(tq + (uint32_t)((2 * sb + hf) * N + NQP + col0), lo[hf]);
+        for (int hf = 0; hf < T; ++hf) ew[hf] = sh.exps[es][hf * kTcTile + my_row];
+        const int vslot = sh.vslot[es];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.efree[es]);
+        q8_wait(&sh.sfull[sb], (i / KS) & 1u, abort_flag, p.err);
+        tc_fence_after();
+        f32x2 x[T][NP];
+        {
+          float hi[T][NL], lo[T][NL];
+#pragma unroll
+          for (int hf = 0; hf < T; ++hf) {
+            tmem_cols<NL>(tq + (uint32_t)((T * sb + hf) * N + col0), hi[hf]);
+            tmem_cols<NL>(tq + (uint32_t)((T * sb + hf) * N + NQP + col0), lo[hf]);
           }
           tc_wait_ld();
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
+          for (int hf = 0; hf < T; ++hf) {
             const float ka = exp2_int((int)(signed char)ew[hf]), kb = exp2_int((int)(signed char)(ew[hf] >> 16));
             const float va = (float)(signed char)(ew[hf] >> 8), vb = (float)(signed char)(ew[hf] >> 24);
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-              const f32x2 s = fma2(pk2(lo[hf][2 * j], lo[hf][2 * j + 1]), c16, pk2(hi[hf][2 * j], hi[hf][2 * j + 1]));
+              const f32x2 y = fma2(pk2(lo[hf][2 * j], lo[hf][2 * j + 1]), c16, pk2(hi[hf][2 * j], hi[hf][2 * j + 1]));
               const float2 cs = *reinterpret_cast<const float2*>(csc + 2 * j);
-              x[hf][j] = fma2(mul2(s, by_head(j, ka, kb)), pk2(cs.x, cs.y), by_head(j, va, vb));
+              x[hf][j] = fma2(mul2(y, by_head(j, ka, kb)), pk2(cs.x, cs.y), by_head(j, va, vb));
             }
           }
           // (after the scales are read: the Q warp may rewrite them once S is free)
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_sfree[sb]);
+          if (lane == 0) mbar_arrive(&sh.sfree[sb]);
         }
-        // masking, as K2: nothing to do on a tile pair inside the unit and below the
-        // causal frontier of the window's first row
-        const int pair_last = k0 + 2 * kTcTile - 1;
-        if (pair_last >= r_hi || col0 + NL > nvec || p.row_pos != nullptr || pair_last > S.k_len - S.q_len) {
+        // masking, as K2: nothing to do on a step inside the unit and below the causal
+        // frontier of the window's first row
+        const int last = k0 + STEP - 1;
+        if (last >= r_hi || col0 + NL > nvec || p.row_pos != nullptr || last > S.k_len - S.q_len) {
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
+          for (int hf = 0; hf < T; ++hf) {
             const int key = k0 + hf * kTcTile + my_row;
             const int nlim = key < r_hi ? nvec : 0;
             const int thr = (key - (S.k_len - S.q_len)) * p.G;
@@ -824,25 +878,30 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int n = col0 + 2 * j + e;
-                const bool see = n < nlim && (p.row_pos != nullptr ? key <= rp[n] : uc.vec(n) >= thr);
+                const bool see = n < nlim && (p.row_pos != nullptr ? key <= sh.rp[n] : uc.vec(n) >= thr);
                 y[e] = see ? y[e] : NEG_INF;
               }
               x[hf][j] = pk2(y[0], y[1]);
             }
           }
         }
-        float* rb = red + (2 * g + ((i / G) & 1u)) * (4 * NQP);
+        float* rb = sh.red[i & 1u][0];
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          float a0, a1, b0, b1;
-          up2(x[0][j], a0, a1);
-          up2(x[1][j], b0, b1);
-          const float r0 = warp_max_f32(fmaxf(a0, b0)), r1 = warp_max_f32(fmaxf(a1, b1));
-          if (lane == 0) *reinterpret_cast<float2*>(rb + sq * NQP + col0 + 2 * j) = make_float2(r0, r1);
+          float m0, m1;
+          up2(x[0][j], m0, m1);
+          if constexpr (T == 2) {
+            float b0, b1;
+            up2(x[1][j], b0, b1);
+            m0 = fmaxf(m0, b0);
+            m1 = fmaxf(m1, b1);
+          }
+          m0 = warp_max_f32(m0);
+          m1 = warp_max_f32(m1);
+          if (lane == 0) *reinterpret_cast<float2*>(rb + sq * NQP + col0 + 2 * j) = make_float2(m0, m1);
         }
-        group_bar();
-        if (t >= G) add_o(i - G);  // relative to the maximum before this pair; also frees P^T
-        float* mw = mxs + sw * 32;
+        softmax_bar<SMT>();
+        if (t >= 1) add_o(i - 1);  // relative to the maximum before this step; also frees P^T
         float al = 1.f;
         if (lane < NL) {
           const int c = col0 + lane;
@@ -864,26 +923,26 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
             oacc[j] = mul2(oacc[j], pk2(aj.x, aj.y));
           }
         }
-        if (pair_last >= r_hi && col0 == 0) {  // warp-uniform
-          // rows past the range may hold anything: once the pair has landed, zero these keys' V rows
-          q8_wait(&bar_vfull[i % VS], (i / VS) & 1u, &s_abort, p.err);
+        if (last >= r_hi && col0 == 0) {  // warp-uniform
+          // rows past the range may hold anything: once the tiles have landed, zero these keys' V rows
+          q8_wait(&sh.vfull[vslot & 255], (uint32_t)(vslot >> 8), abort_flag, p.err);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
+          for (int hf = 0; hf < T; ++hf) {
             if (k0 + hf * kTcTile + my_row >= r_hi) {
-              unsigned char* vrow = vts + (int)(i % VS) * C::PAIR_BYTES + (hf * kTcTile + my_row) * 128;
+              unsigned char* vrow = vts + (vslot & 255) * C::STEP_BYTES + (hf * kTcTile + my_row) * 128;
 #pragma unroll
               for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vrow + c * 16) = make_uint4(0, 0, 0, 0);
             }
           }
         }
         // weights 2^(t - M + 8); the denominator's leave the value scale out again.
-        // (A pair of one tile: the other's are zero, and no MMA reads them.)
-        uint32_t w1[2][(NL + 3) / 4], w2[2][(NL + 3) / 4];
+        // (A step of one tile: the other's are zero, and no MMA reads them.)
+        uint32_t w1[T][(NL + 3) / 4], w2[T][(NL + 3) / 4];
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
           const float2 mj = *reinterpret_cast<const float2*>(mw + 2 * j);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
+          for (int hf = 0; hf < T; ++hf) {
             const float ia = exp2_int(-(int)(signed char)(ew[hf] >> 8)), ib = exp2_int(-(int)(signed char)(ew[hf] >> 24));
             float d0, d1;
             up2(add2(x[hf][j], pk2(mj.x, mj.y)), d0, d1);
@@ -901,33 +960,31 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
           }
         }
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < T; ++hf) {
           const uint32_t rowo = (uint32_t)((hf * kTcTile + my_row) * C::P_ROWB);
           auto put = [&](int col, const uint32_t(&w)[(NL + 3) / 4]) {
             uint32_t off = rowo + (uint32_t)col;
             off ^= ((off >> 7) & ((1u << C::P_SWZ_BITS) - 1u)) << 4;
             if constexpr (NL == 16)
-              *reinterpret_cast<uint4*>(pg + off) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(ps + off) = make_uint4(w[0], w[1], w[2], w[3]);
             else if constexpr (NL == 8)
-              *reinterpret_cast<uint2*>(pg + off) = make_uint2(w[0], w[1]);
+              *reinterpret_cast<uint2*>(ps + off) = make_uint2(w[0], w[1]);
             else if constexpr (NL == 4)
-              *reinterpret_cast<uint32_t*>(pg + off) = w[0];
+              *reinterpret_cast<uint32_t*>(ps + off) = w[0];
             else
-              *reinterpret_cast<uint16_t*>(pg + off) = (uint16_t)w[0];
+              *reinterpret_cast<uint16_t*>(ps + off) = (uint16_t)w[0];
           };
           put(col0, w1[hf]);
           put(NQP + col0, w2[hf]);
         }
         fence_async_smem();
-        group_bar();
-        if (stid == 0) mbar_arrive(&bar_pfull[g]);
+        softmax_bar<SMT>();
+        if (stid == 0) mbar_arrive(&sh.pfull);
       }
-      if (t0 < n_t) add_o(it + (uint32_t)(t0 + (n_t - 1 - t0) / G * G));
-      it += n_t;
-      ++units;
+      add_o(s.step + (uint32_t)n_t - 1);
 
       // ---- column sums of the weights over the unit's keys
-      float* lb = lred + (2 * g + (units & 1u)) * (4 * NQP);
+      float* lb = sh.lred[s.unit & 1u][0];
       {
         float w[NL];
 #pragma unroll
@@ -935,44 +992,11 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
         const float r = warp_col_sum<NL>(w, lane);
         if (lane < NL) lb[sq * NQP + col0 + reduced_col<NL>(lane)] = r;
       }
-      group_bar();
-      float mc[NL], lc[NL], oc[NL];
-#pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const int n = col0 + j;
-        mc[j] = __shfl_sync(0xffffffffu, m, j);
-        lc[j] = lb[n] + lb[NQP + n] + lb[2 * NQP + n] + lb[3 * NQP + n];
-      }
+      softmax_bar<SMT>();
+      float oc[NL];
 #pragma unroll
       for (int j = 0; j < NP; ++j) up2(oacc[j], oc[2 * j], oc[2 * j + 1]);
-      if constexpr (G == 2) {
-        // the second group hands its (m, l, O) over through shared memory (O in its own
-        // P^T buffer, whose last P.V is done) and goes on to the next unit
-        float* og = reinterpret_cast<float*>(ps + C::P_BYTES);
-        if (g == 1) {
-#pragma unroll
-          for (int j = 0; j < NL; ++j) {
-            og[j * kTcTile + my_row] = oc[j];
-            if (my_row == 0) {
-              ml[j] = mc[j];
-              ml[NQP + j] = lc[j];
-            }
-          }
-        }
-        all_bar();
-        if (g == 0) {
-#pragma unroll
-          for (int j = 0; j < NL; ++j) {
-            const float m1 = ml[j], nm = fmaxf(mc[j], m1), ms = nm == NEG_INF ? 0.f : nm;
-            const float wa = ex2_ftz(mc[j] - ms), wb = ex2_ftz(m1 - ms);
-            lc[j] = lc[j] * wa + ml[NQP + j] * wb;
-            oc[j] = oc[j] * wa + og[j * kTcTile + my_row] * wb;
-            mc[j] = nm;
-          }
-        }
-        all_bar();
-        if (g == 1) continue;
-      }
+      auto lsum = [&](int n) { return lb[n] + lb[NQP + n] + lb[2 * NQP + n] + lb[3 * NQP + n]; };
       const int dim = my_row;
       // output element of query column n held by this thread's O^T row, or -1
       auto out_at = [&](int n) -> long long {
@@ -988,84 +1012,79 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), 1)
       if (n_contrib == 1) {
 #pragma unroll
         for (int j = 0; j < NL; ++j)
-          if (col0 + j < nvec) put_out(col0 + j, oc[j], lc[j]);
+          if (col0 + j < nvec) put_out(col0 + j, oc[j], lsum(col0 + j));
       } else {
-        if (!itr.waited) {
+        if (!s.waited) {
           griddep_wait();
-          itr.waited = true;
+          s.waited = true;
         }
-        // 2: every other contributor had published when this CTA began the unit
+        // 2: every other contributor had published when this stream began the unit
         if (stid == 0) {
-          s_flag = (arrived == n_contrib - 1) ? 2 : 0;
-          if (s_flag == 2) fence_acq_rel_gpu();
+          sh.flag = (arrived == n_contrib - 1) ? 2 : 0;
+          if (sh.flag == 2) fence_acq_rel_gpu();
         }
-        group_bar();
-        if (s_flag != 2) {
-          const int slot = (ustart < a) ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
+        softmax_bar<SMT>();
+        if (sh.flag != 2) {
+          const int slot = (ustart < a) ? 2 * vid : 2 * vid + 1;
           float* pb = p.ws_part + (size_t)slot * C::PART_FLOATS;
 #pragma unroll
           for (int j = 0; j < NL; ++j) {
+            const float mj = __shfl_sync(0xffffffffu, m, j);
             if (col0 + j < nvec) {
               if (dim == 0) {
-                pb[col0 + j] = mc[j];
-                pb[NQP + col0 + j] = lc[j];
+                pb[col0 + j] = mj;
+                pb[NQP + col0 + j] = lsum(col0 + j);
               }
               pb[2 * NQP + (col0 + j) * 128 + dim] = oc[j];
             }
           }
           __threadfence();
-          group_bar();
+          softmax_bar<SMT>();
           if (stid == 0) {
             const int prev = atomicAdd(p.ws_cnt + c_first, 1);
-            s_flag = (prev == n_contrib - 1) ? 1 : 0;
+            sh.flag = (prev == n_contrib - 1) ? 1 : 0;
           }
-          group_bar();
+          softmax_bar<SMT>();
         }
-        if (s_flag) {
+        if (sh.flag) {
           __threadfence();
-          // online merge in key order, whoever arrives last
-          const int k_own = (int)blockIdx.x - c_first;
-          float M[NL], Ls[NL], acc[NL];
+          // online merge in key order, whoever arrives last; a column at a time (the
+          // loads of one contributor are independent)
+          const int k_own = vid - c_first;
 #pragma unroll
           for (int j = 0; j < NL; ++j) {
-            M[j] = NEG_INF;
-            Ls[j] = 0.f;
-            acc[j] = 0.f;
-          }
-          for (int k = 0; k < n_contrib; ++k) {
-            const int cc = c_first + k;
-            const float* base = p.ws_part + (size_t)(k == 0 ? 2 * cc + 1 : 2 * cc) * C::PART_FLOATS;
-            float mk[NL], lk[NL], ok[NL];
-#pragma unroll
-            for (int j = 0; j < NL; ++j) {
-              const int n = col0 + j;
-              if (k == k_own) {
-                mk[j] = mc[j];
-                lk[j] = lc[j];
-                ok[j] = oc[j];
-              } else {
-                mk[j] = n < nvec ? ld_cg_f32(base + n) : NEG_INF;
-                lk[j] = n < nvec ? ld_cg_f32(base + NQP + n) : 0.f;
-                ok[j] = n < nvec ? ld_cg_f32(base + 2 * NQP + n * 128 + dim) : 0.f;
+            const int n = col0 + j;
+            const float mj = __shfl_sync(0xffffffffu, m, j);
+            if (n < nvec) {
+              float M = NEG_INF, Ls = 0.f, acc = 0.f;
+              for (int k = 0; k < n_contrib; ++k) {
+                const int cc = c_first + k;
+                const float* base = p.ws_part + (size_t)(k == 0 ? 2 * cc + 1 : 2 * cc) * C::PART_FLOATS;
+                float mk = mj, lk, ok = oc[j];
+                if (k == k_own) {
+                  lk = lsum(n);
+                } else {
+                  mk = ld_cg_f32(base + n);
+                  lk = ld_cg_f32(base + NQP + n);
+                  ok = ld_cg_f32(base + 2 * NQP + n * 128 + dim);
+                }
+                const float nm = fmaxf(M, mk);
+                const float ms = nm == NEG_INF ? 0.f : nm;
+                const float wa = fast_exp2(M - ms), wb = fast_exp2(mk - ms);
+                Ls = Ls * wa + lk * wb;
+                acc = acc * wa + ok * wb;
+                M = nm;
               }
-            }
-#pragma unroll
-            for (int j = 0; j < NL; ++j) {
-              const float nm = fmaxf(M[j], mk[j]);
-              const float ms = nm == NEG_INF ? 0.f : nm;
-              const float wa = fast_exp2(M[j] - ms), wb = fast_exp2(mk[j] - ms);
-              Ls[j] = Ls[j] * wa + lk[j] * wb;
-              acc[j] = acc[j] * wa + ok[j] * wb;
-              M[j] = nm;
+              put_out(n, acc, Ls);
             }
           }
-#pragma unroll
-          for (int j = 0; j < NL; ++j)
-            if (col0 + j < nvec) put_out(col0 + j, acc[j], Ls[j]);
         }
-        if (s_flag && stid == 0) p.ws_cnt[c_first] = 0;
-        group_bar();  // s_flag is rewritten by the next unit
+        if (sh.flag && stid == 0) p.ws_cnt[c_first] = 0;
+        softmax_bar<SMT>();  // s_flag is rewritten by the next unit
       }
+      s.step += (uint32_t)n_t;
+      ++s.unit;
+      s.next_unit(p, STEP);
     }
   }
 
