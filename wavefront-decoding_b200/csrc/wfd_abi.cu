@@ -1601,7 +1601,8 @@ extern "C" int wfd_wave_attn_q8(int32_t which, const wfd_q8_cache* cache, const 
   pp.q8 = c;
   pp.zero = reinterpret_cast<int*>(ws + L.cnt);
   pp.n_zero = 2 * sms;
-  pp.min_share = kQ8MinShare;
+  pp.min_share = which == 1 ? 1 : kQ8MinShare;
+  pp.chunk = which == 1 ? kQ8Chunk256 : 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 plan_grid(1 + (n_items < 4 * sms ? n_items : 4 * sms));
   const cudaError_t pe = dtype == WFD_DTYPE_BF16

@@ -66,7 +66,8 @@ struct PlanParams {
   // window append into an 8-bit cache (plan_kernel<T>: k_new / v_new hold T rows);
   // its slots and the items' are both counted from the call's slot offset
   Q8Cache q8;
-  int min_share;  // plan_kernel<T>: smallest share of a CTA (0: none)
+  int min_share;  // plan_kernel<T>: smallest share of a CTA
+  int chunk;      // plan_kernel<T>: keys that count as one (work is counted in chunks of a unit)
   int* zero;  // plan_kernel<T>: arrival counters cleared for the attention (n_zero)
   int n_zero;
 };
@@ -270,6 +271,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       const long long qv = (long long)s.q_len * p.G;
       s.n_qg = (qv == 0) ? 0 : (p.qg_split ? (int)((qv + p.NQ - 1) / p.NQ) : 1);
       work = (long long)s.n_qg * s.k_len;
+      if constexpr (!std::is_void<TQ>::value) work = (long long)s.n_qg * ((s.k_len + p.chunk - 1) / p.chunk);
       p.segs[i] = s;
       // Query rows with no key to attend produce zeros (written here; no
       // attention CTA visits a zero-work segment).

@@ -196,13 +196,20 @@ __device__ __forceinline__ void q8_split(f32x2 w, uint32_t& p1, uint32_t& p2) {
   p2 = e4m3x2(a, b);
 }
 
-// A CTA's walk over its share [pos, end) of the work: the pieces [r_lo, r_hi) of
-// units (segment, query group, kv head), in order, as UnitIter's; a unit that follows
-// in the same segment costs no division and no load.
+// Work is counted in chunks of 256 keys of a unit (segment, query group, kv head),
+// the last of a unit possibly shorter: a piece of a few keys takes as long as a whole
+// step and is one more to merge, so units are cut at chunk borders only.  (Shares in
+// keys, as K2's, took 36 us for 256 units of 65 keys, chunks 22 us.)
+constexpr int kQ8Chunk256 = 256;
+__device__ __forceinline__ int q8_chunks(int k_len) { return (k_len + kQ8Chunk256 - 1) / kQ8Chunk256; }
+
+// A CTA's walk over its share [pos, end) of the work, in chunks: the pieces [r_lo,
+// r_hi) (keys) of units, in order; a unit that follows in the same segment costs no
+// division and no load.
 struct Q8Stream {
   long long pos, end, base, nbase, ustart;
   Seg S;
-  int seg, u, r_lo, r_hi;
+  int seg, u, uc, r_lo, r_hi;  // uc: chunks of a unit of this segment
   int t, n;        // step of the piece, steps of the piece
   uint32_t step, unit;  // steps and units so far (the current one not counted)
   bool fresh;      // u not yet known in this segment
@@ -232,14 +239,15 @@ struct Q8Stream {
         fresh = true;
       }
       if (fresh) {
-        u = pos == base ? 0 : (int)((pos - base) / S.k_len);
-        ustart = base + (long long)u * S.k_len;
+        uc = q8_chunks(S.k_len);
+        u = pos == base ? 0 : (int)((pos - base) / uc);
+        ustart = base + (long long)u * uc;
         fresh = false;
       } else {
         ++u;
-        ustart += S.k_len;
+        ustart += uc;
       }
-      const long long uend = ustart + S.k_len;
+      const long long uend = ustart + uc;
       if (p.invariant) {
         const bool mine = ustart >= pos;  // else it began in the share before this one, which takes it whole
         pos = uend;
@@ -247,9 +255,9 @@ struct Q8Stream {
         r_lo = 0;
         r_hi = S.k_len;
       } else {
-        r_lo = (int)(pos - ustart);
-        r_hi = (int)((uend < end ? uend : end) - ustart);
-        pos = ustart + r_hi;
+        r_lo = (int)(pos - ustart) * kQ8Chunk256;
+        pos = uend < end ? uend : end;
+        r_hi = min(S.k_len, (int)(pos - ustart) * kQ8Chunk256);
       }
       t = 0;
       n = (r_hi - r_lo + step_keys - 1) / step_keys;
@@ -274,7 +282,7 @@ struct SelfStart {
   int seg0, slot0, seq0, minpos;
 };
 __device__ __forceinline__ void share_of(long long total, long long& share, long long& a, long long& b) {
-  share = max((total + gridDim.x - 1) / gridDim.x, (long long)kQ8MinShare);
+  share = max((total + gridDim.x - 1) / gridDim.x, 1ll);
   a = min(total, (long long)blockIdx.x * share);
   b = min(total, a + share);
 }
@@ -292,7 +300,8 @@ __device__ __forceinline__ void self_start(const VerifyParams& p, SelfStart& sh,
     if (i < p.n_segs) {
       my[k] = p.items[i];
       Seg s;
-      w[k] = slot_segment(p, my[k], s);
+      slot_segment(p, my[k], s);
+      w[k] = (long long)s.n_qg * q8_chunks(s.k_len);
     }
     tsum += w[k];
   }
@@ -658,30 +667,34 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
     while (s.live) {
       const int h = s.u % p.Hkv, qg = s.u / p.Hkv;
       const uint32_t w = s.unit, qb = w % QB;
+      const UnitCols<PAIR, NQP> uc(p, s.S, qg);
+      unsigned char* qd = qs + qb * C::Q_BYTES;
+      float* cd = sh.cscale[w & 3u];
+      constexpr int NB = NA < 8 ? NA : 8;  // vectors loaded at once
+      uint2 raw[NB];
+      auto load = [&](int n0) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int n = n0 + i;
+          raw[i] = make_uint2(0, 0);
+          if (n < uc.nvec) {
+            const int e = uc.head(n), v = uc.vec(n);
+            const long long row = (long long)(s.S.q_row0 + v / p.G) * p.Hq + v % p.G;
+            if (PAIR) {
+              if ((lane >> 4) == e)
+                raw[i] = *reinterpret_cast<const uint2*>(q + (row + (2 * h + e) * p.G) * 64 + (lane & 15) * 4);
+            } else {
+              raw[i] = *reinterpret_cast<const uint2*>(q + (row + h * p.G) * 128 + lane * 4);
+            }
+          }
+        }
+      };
+      load(0);  // on its way while the buffer is still in use
       bool go = w >= (uint32_t)QB ? q8_wait(&sh.qfree[qb], ((w / QB) - 1) & 1u, abort_flag, p.err) : !*abort_flag;
       go = __all_sync(0xffffffffu, go);
       if (go) {
-        const UnitCols<PAIR, NQP> uc(p, s.S, qg);
-        unsigned char* qd = qs + qb * C::Q_BYTES;
-        float* cd = sh.cscale[w & 3u];
-        constexpr int NB = NA < 8 ? NA : 8;  // vectors loaded at once
         for (int n0 = 0; n0 < NA; n0 += NB) {
-          uint2 raw[NB];
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const int n = n0 + i;
-            raw[i] = make_uint2(0, 0);
-            if (n < uc.nvec) {
-              const int e = uc.head(n), v = uc.vec(n);
-              const long long row = (long long)(s.S.q_row0 + v / p.G) * p.Hq + v % p.G;
-              if (PAIR) {
-                if ((lane >> 4) == e)
-                  raw[i] = *reinterpret_cast<const uint2*>(q + (row + (2 * h + e) * p.G) * 64 + (lane & 15) * 4);
-              } else {
-                raw[i] = *reinterpret_cast<const uint2*>(q + (row + h * p.G) * 128 + lane * 4);
-              }
-            }
-          }
+          if (n0 > 0) load(n0);
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             const int n = n0 + i;
@@ -786,7 +799,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
       if (nvec > NA && stid == 0) set_error(p.err, kErrBadRows);  // an item longer than the call's max_q
       // the shares that hold keys of this unit
       const int c_first = ustart >= a ? vid : (int)(ustart / share);
-      const int c_last = ustart + S.k_len <= a + share ? vid : (int)((ustart + S.k_len - 1) / share);
+      const int c_last = ustart + s.uc <= a + share ? vid : (int)((ustart + s.uc - 1) / share);
       const int n_contrib = p.invariant ? 1 : c_last - c_first + 1;
       int arrived = 0;
       // (the plan kernel clears the counters, so they are read after it only)
@@ -1048,35 +1061,49 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
         }
         if (sh.flag) {
           __threadfence();
-          // online merge in key order, whoever arrives last; a column at a time (the
-          // loads of one contributor are independent)
+          // online merge in key order, whoever arrives last; up to 8 columns at a time,
+          // whose loads of one contributor are all in flight together
           const int k_own = vid - c_first;
+          constexpr int MC = NL < 8 ? NL : 8;
 #pragma unroll
-          for (int j = 0; j < NL; ++j) {
-            const int n = col0 + j;
-            const float mj = __shfl_sync(0xffffffffu, m, j);
-            if (n < nvec) {
-              float M = NEG_INF, Ls = 0.f, acc = 0.f;
-              for (int k = 0; k < n_contrib; ++k) {
-                const int cc = c_first + k;
-                const float* base = p.ws_part + (size_t)(k == 0 ? 2 * cc + 1 : 2 * cc) * C::PART_FLOATS;
-                float mk = mj, lk, ok = oc[j];
-                if (k == k_own) {
-                  lk = lsum(n);
-                } else {
-                  mk = ld_cg_f32(base + n);
-                  lk = ld_cg_f32(base + NQP + n);
-                  ok = ld_cg_f32(base + 2 * NQP + n * 128 + dim);
-                }
-                const float nm = fmaxf(M, mk);
-                const float ms = nm == NEG_INF ? 0.f : nm;
-                const float wa = fast_exp2(M - ms), wb = fast_exp2(mk - ms);
-                Ls = Ls * wa + lk * wb;
-                acc = acc * wa + ok * wb;
-                M = nm;
-              }
-              put_out(n, acc, Ls);
+          for (int j0 = 0; j0 < NL; j0 += MC) {
+            float M[MC], Ls[MC], acc[MC];
+#pragma unroll
+            for (int j = 0; j < MC; ++j) {
+              M[j] = NEG_INF;
+              Ls[j] = acc[j] = 0.f;
             }
+            for (int k = 0; k < n_contrib; ++k) {
+              const int cc = c_first + k;
+              const float* base = p.ws_part + (size_t)(k == 0 ? 2 * cc + 1 : 2 * cc) * C::PART_FLOATS;
+              float mk[MC], lk[MC], ok[MC];
+#pragma unroll
+              for (int j = 0; j < MC; ++j) {
+                const int n = col0 + j0 + j;
+                const float mj = __shfl_sync(0xffffffffu, m, j0 + j);
+                mk[j] = mj;
+                lk[j] = 0.f;
+                ok[j] = oc[j0 + j];
+                if (k != k_own && n < nvec) {
+                  mk[j] = ld_cg_f32(base + n);
+                  lk[j] = ld_cg_f32(base + NQP + n);
+                  ok[j] = ld_cg_f32(base + 2 * NQP + n * 128 + dim);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < MC; ++j) {
+                if (k == k_own) lk[j] = lsum(col0 + j0 + j);
+                const float nm = fmaxf(M[j], mk[j]);
+                const float ms = nm == NEG_INF ? 0.f : nm;
+                const float wa = fast_exp2(M[j] - ms), wb = fast_exp2(mk[j] - ms);
+                Ls[j] = Ls[j] * wa + lk[j] * wb;
+                acc[j] = acc[j] * wa + ok[j] * wb;
+                M[j] = nm;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < MC; ++j)
+              if (col0 + j0 + j < nvec) put_out(col0 + j0 + j, acc[j], Ls[j]);
           }
         }
         if (sh.flag && stid == 0) p.ws_cnt[c_first] = 0;
