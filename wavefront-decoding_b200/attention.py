@@ -191,8 +191,9 @@ def wave_attn(q, k_new, v_new, k_cache, v_cache, items, max_q: int, *, lens=None
 def wave_attn_q8(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q: int, *, lens=None,
                  slot_offset: int = 0, out: torch.Tensor | None = None, scale: float | None = None, kernel: int = -1,
                  row_pos: torch.Tensor | None = None):
-    """wave_attn over an 8-bit slot cache (kv_cache.QuantKVCache), through the
-    dispatcher op torch.ops.wfd.wave_attn_q8 (wave_attn_q8_out with `out`).
+    """wave_attn over an 8-bit slot cache (kv_cache.QuantKVCache): the dispatcher op
+    torch.ops.wfd.wave_attn_q8 (wave_attn_q8_out with `out`), or its kernel directly
+    where no tracing or dispatch mode is active.
 
     k_cache / v_cache: float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) codes;
     k_exp / v_exp: int8 (n_slots, n_seqs, Hkv, max_seq); a cached value is code *
@@ -202,10 +203,15 @@ def wave_attn_q8(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q: 
     and row_pos as in wave_attn.  kernel: -1 auto, 0 CUDA cores (fp32, and bf16 at
     head_dim 64 with an odd kv-head count), 1 tcgen05.  Uses no shared workspace:
     calls on several streams do not disturb each other."""
-    rt.require_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items)
+    if not q.is_cuda:
+        rt.require_cuda(q)
+    args = (q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, int(max_q), lens, int(slot_offset), scale,
+            int(kernel), row_pos)
+    if _ops.plain_eager(q):   # nothing traces or dispatches on the call: the op's kernel without the dispatcher (11 us)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        _ops._wave_attn_q8_out_cuda(*args, out)
+        return out
     if out is None:
-        return torch.ops.wfd.wave_attn_q8(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, int(max_q), lens,
-                                          int(slot_offset), scale, int(kernel), row_pos)
-    torch.ops.wfd.wave_attn_q8_out(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, int(max_q), lens,
-                                   int(slot_offset), scale, int(kernel), row_pos, out)
+        return torch.ops.wfd.wave_attn_q8(*args)
+    torch.ops.wfd.wave_attn_q8_out(*args, out)
     return out

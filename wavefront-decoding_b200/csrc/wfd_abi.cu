@@ -1459,16 +1459,16 @@ extern "C" int wfd_write_prefill_q8(const wfd_q8_cache* cache, const void* k, co
   if (!k || !v) return WFD_ERR_INVALID_ARG;
   if (!aligned16(k) || !aligned16(v)) return WFD_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((L + kQ8Chunk - 1) / kQ8Chunk, c.n_seqs, 2);
-  const size_t smem = (size_t)c.Hkv * kQ8Chunk;
+  const int parts = (c.Hkv * c.Dh + kQ8Span - 1) / kQ8Span, log2_dh = __builtin_ctz((unsigned)c.Dh);
+  const dim3 grid((L + kQ8Chunk - 1) / kQ8Chunk, c.n_seqs, 2 * parts);
   cudaError_t e;
   if (dtype == WFD_DTYPE_BF16)
-    e = launch_pdl(q8_prefill_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), smem, st,
+    e = launch_pdl(q8_prefill_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), 0, st,
                    static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), c, cache->lens, slot, L,
-                   d_err);
+                   log2_dh, d_err);
   else
-    e = launch_pdl(q8_prefill_kernel<float>, grid, dim3(kQ8Threads), smem, st, static_cast<const float*>(k),
-                   static_cast<const float*>(v), c, cache->lens, slot, L, d_err);
+    e = launch_pdl(q8_prefill_kernel<float>, grid, dim3(kQ8Threads), 0, st, static_cast<const float*>(k),
+                   static_cast<const float*>(v), c, cache->lens, slot, L, log2_dh, d_err);
   return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
 }
 
@@ -1487,17 +1487,17 @@ extern "C" int wfd_gather_q8(const wfd_q8_cache* cache, void* k_pack, void* v_pa
   if (sms <= 0) return WFD_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int chunks = (c.max_seq + kQ8Chunk - 1) / kQ8Chunk;
-  const int want = 32 * sms / (2 * n) + 1;  // lengths are device data: enough blocks to fill the GPU for any
-  const dim3 grid(chunks < want ? chunks : want, n, 2);
-  const size_t smem = (size_t)c.Hkv * kQ8Chunk;
+  const int parts = (c.Hkv * c.Dh + kQ8Span - 1) / kQ8Span, log2_dh = __builtin_ctz((unsigned)c.Dh);
+  const int want = 64 * sms / (2 * parts * n) + 1;  // lengths are device data: enough blocks to fill the GPU for any
+  const dim3 grid(chunks < want ? chunks : want, n, 2 * parts);
   cudaError_t e;
   if (dtype == WFD_DTYPE_BF16)
-    e = launch_pdl(q8_gather_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), smem, st, c,
+    e = launch_pdl(q8_gather_kernel<__nv_bfloat16>, grid, dim3(kQ8Threads), 0, st, c,
                    static_cast<__nv_bfloat16*>(k_pack), static_cast<__nv_bfloat16*>(v_pack), slots, seqs, cu_k,
-                   (long long)total, d_err);
+                   (long long)total, log2_dh, d_err);
   else
-    e = launch_pdl(q8_gather_kernel<float>, grid, dim3(kQ8Threads), smem, st, c, static_cast<float*>(k_pack),
-                   static_cast<float*>(v_pack), slots, seqs, cu_k, (long long)total, d_err);
+    e = launch_pdl(q8_gather_kernel<float>, grid, dim3(kQ8Threads), 0, st, c, static_cast<float*>(k_pack),
+                   static_cast<float*>(v_pack), slots, seqs, cu_k, (long long)total, log2_dh, d_err);
   return e == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
 }
 

@@ -54,20 +54,36 @@ __device__ __forceinline__ void e4m3x4_to_f(uint32_t w, float (&f)[4]) {
 }
 
 // Quantise the row held by this thread's group of `lanes` neighbouring lanes (a
-// power of two; every lane of the warp calls), 8 values each.
-__device__ __forceinline__ uint2 q8_quantise(float (&f)[8], int lanes, int& e, bool& nan) {
-  float a = 0.f;
-  nan = false;
+// power of two; every lane of the warp calls), 8 values each.  The largest |x| is
+// found as an integer: a NaN's bits lie above those of infinity, so the same maximum
+// tells whether the row holds one.
+__device__ __forceinline__ uint32_t q8_max_bits(const float (&f)[8]) {
+  uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (isnan(f[i])) {
-      nan = true;
-      f[i] = 0.f;
+  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(f[i]) & 0x7fffffffu);
+  return a;
+}
+// ... of 8 packed bf16 (a NaN comes out as one)
+__device__ __forceinline__ uint32_t q8_max_bits(const uint4& w) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+  return max(u << 16, u & 0xffff0000u) & 0x7fffffffu;
+}
+// a: q8_max_bits of f
+__device__ __forceinline__ uint2 q8_quantise(float (&f)[8], uint32_t a, int lanes, int& e, bool& nan) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  nan = a > 0x7f800000u;
+  if (__any_sync(0xffffffffu, nan)) {
+    a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (isnan(f[i])) f[i] = 0.f;
+      a = max(a, __float_as_uint(f[i]) & 0x7fffffffu);
     }
-    a = fmaxf(a, fabsf(f[i]));
+    for (int o = lanes >> 1; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
   }
-  for (int o = lanes >> 1; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  e = max(-kQ8ExpMax, min(kQ8ExpMax, q8_exponent(a)));
+  e = max(-kQ8ExpMax, min(kQ8ExpMax, q8_exponent(__uint_as_float(a))));
   const float s = exp2_int(-e);
   uint2 q;
   q.x = e4m3x2(f[0] * s, f[1] * s) | (e4m3x2(f[2] * s, f[3] * s) << 16);
@@ -108,7 +124,7 @@ __device__ __forceinline__ void q8_put_rows(const T* k_new, const T* v_new, long
     if (pos >= 0) Vec8<T>::load((isv ? v_new : k_new) + (src_row0 + j) * width + x, f);
     int ex;
     bool nan;
-    const uint2 q = q8_quantise(f, lanes, ex, nan);
+    const uint2 q = q8_quantise(f, q8_max_bits(f), lanes, ex, nan);
     if (pos >= 0) {
       *reinterpret_cast<uint2*>((isv ? c.v : c.k) + c.row(slot, seq, pos) + x) = q;
       const int h = x / c.Dh;
@@ -145,114 +161,141 @@ __global__ void q8_append_kernel(const T* k_new, const T* v_new, const Q8Cache c
   if (threadIdx.x == 0 && lens != nullptr) atomicMax(lens + (long long)slot * c.n_seqs + seq, pos + 1);
 }
 
-// Positions handled by one block of the prompt write and of the read-back: their
-// exponents (one byte per head and position, 32 contiguous) pass through shared
-// memory, so that they are read and written as whole 32-byte sectors.
+// The prompt write and the read-back move blocks of 32 positions x up to 512 values
+// of the row (8 heads of 64, 4 of 128): their exponents, one byte per head and
+// position, 32 of a head contiguous, pass through shared memory, so that they are
+// read and written as whole 32-byte sectors, and blocks are small enough that a
+// single prompt fills the GPU.  A thread keeps its place in the row and steps through
+// the positions; all its loads are in flight before the first is used.  (Prompt of
+// 64 x 1024 x 24 x 64, bf16: WRITEUS us written, READUS us read back, 92 us each of HBM
+// time; whole rows a block, with divisions by the head count: 167 and 103.)
 constexpr int kQ8Chunk = 32;
 constexpr int kQ8Threads = 256;
-constexpr int kQ8MaxHeads = 1024;  // kv heads (shared memory of one chunk's exponents: 32 KB)
+constexpr int kQ8MaxHeads = 1024;  // kv heads
+constexpr int kQ8Span = 512;       // values of a row per block
+constexpr int kQ8Heads = kQ8Span / 16;  // heads per block, at most
 
 // write_prefill: k, v (n_seqs, L, Hkv, Dh) -> positions [0, L) of `slot`.
-// Block (chunk, sequence, K or V).
+// Block (chunk, sequence, part of the row of K or V).
 template <typename T>
 __global__ void __launch_bounds__(kQ8Threads)
-    q8_prefill_kernel(const T* k, const T* v, const Q8Cache c, int32_t* lens, int slot, int L, int* err) {
+    q8_prefill_kernel(const T* k, const T* v, const Q8Cache c, int32_t* lens, int slot, int L, int log2_dh, int* err) {
   griddep_wait();
-  extern __shared__ int8_t s_exp[];  // [Hkv][kQ8Chunk]
+  __shared__ int8_t s_exp[kQ8Heads][kQ8Chunk];
   const int p0 = blockIdx.x * kQ8Chunk, seq = blockIdx.y;
-  const bool isv = blockIdx.z != 0;
+  const bool isv = (blockIdx.z & 1) != 0;
+  const int width = c.Hkv * c.Dh;
+  const int x0 = (blockIdx.z >> 1) * kQ8Span;
   const int np = min(kQ8Chunk, L - p0);
-  const int lanes = c.Dh >> 3, width = c.Hkv * c.Dh;
-  const T* src = (isv ? v : k) + ((long long)seq * L + p0) * width;
-  uint8_t* dst = (isv ? c.v : c.k) + c.row(slot, seq, p0);
-  const int units = np * c.Hkv * lanes;
-  constexpr int U = 4;  // rows' loads in flight per thread
-  bool any_nan = false;
-  for (int e0 = 0; e0 < units; e0 += U * kQ8Threads) {
-    float f[U][8];
+  const int lanes = c.Dh >> 3;
+  constexpr int PER = kQ8Span / 8;                 // threads of one position
+  constexpr int STEP = kQ8Threads / PER;           // positions a pass
+  constexpr int U = kQ8Chunk / STEP;
+  const int xi = (threadIdx.x % PER) * 8, x = x0 + xi, j0 = threadIdx.x / PER;
+  const bool on = x < width;
+  const T* src = (isv ? v : k) + ((long long)seq * L + p0) * width + x;
+  uint8_t* dst = (isv ? c.v : c.k) + c.row(slot, seq, p0) + x;
+  constexpr int NV = (int)sizeof(T) / 2;  // 16-byte vectors of 8 values
+  uint4 raw[U][NV];                        // kept as loaded: unpacked, the rows would take twice the registers
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kQ8Threads + threadIdx.x;
+  for (int u = 0; u < U; ++u) {
+    const int j = j0 + u * STEP;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
-      if (e < units) Vec8<T>::load(src + (long long)e * 8, f[u]);
+    for (int i = 0; i < NV; ++i) {
+      raw[u][i] = make_uint4(0, 0, 0, 0);
+      if (on && j < np) raw[u][i] = ld_nc_v4(reinterpret_cast<const uint4*>(src + (long long)j * width) + i);
     }
+  }
+  bool any_nan = false;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kQ8Threads + threadIdx.x;
-      int ex;
-      bool nan;
-      const uint2 q = q8_quantise(f[u], lanes, ex, nan);
-      if (e < units) {
-        *reinterpret_cast<uint2*>(dst + (long long)e * 8) = q;
-        const int hr = e / lanes;  // head row: position * Hkv + head
-        if (hr * lanes == e) s_exp[(hr % c.Hkv) * kQ8Chunk + hr / c.Hkv] = (int8_t)ex;
-        any_nan |= nan;
-      }
+  for (int u = 0; u < U; ++u) {
+    const int j = j0 + u * STEP;
+    int ex;
+    bool nan;
+    float f[8];
+    constexpr int EV = 8 / NV;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float part[EV];
+      Elem<T>::unpack(raw[u][i], part);
+#pragma unroll
+      for (int e = 0; e < EV; ++e) f[i * EV + e] = part[e];
+    }
+    uint32_t a;
+    if constexpr (NV == 1)
+      a = q8_max_bits(raw[u][0]);
+    else
+      a = q8_max_bits(f);
+    const uint2 q = q8_quantise(f, a, lanes, ex, nan);
+    if (on && j < np) {
+      *reinterpret_cast<uint2*>(dst + (long long)j * width) = q;
+      if ((xi & (c.Dh - 1)) == 0) s_exp[xi >> log2_dh][j] = (int8_t)ex;
+      any_nan |= nan;
     }
   }
   if (any_nan) set_error(err, kErrNaN);
   __syncthreads();
-  int8_t* edst = (isv ? c.ve : c.ke) + c.exps(slot, seq) + p0;
-  for (int t = threadIdx.x; t < c.Hkv * kQ8Chunk; t += kQ8Threads) {
+  const int h0 = x0 >> log2_dh, nh = min(kQ8Span, width - x0) >> log2_dh;
+  int8_t* edst = (isv ? c.ve : c.ke) + c.exps(slot, seq) + (long long)h0 * c.max_seq + p0;
+  for (int t = threadIdx.x; t < nh * kQ8Chunk; t += kQ8Threads) {
     const int h = t / kQ8Chunk, j = t % kQ8Chunk;
-    if (j < np) edst[(long long)h * c.max_seq + j] = s_exp[t];
+    if (j < np) edst[(long long)h * c.max_seq + j] = s_exp[h][j];
   }
-  if (lens != nullptr && blockIdx.x == 0 && !isv && threadIdx.x == 0)
+  if (lens != nullptr && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0)
     atomicMax(lens + (long long)slot * c.n_seqs + seq, L);
 }
 
 // Read back: segment i dequantises positions [0, cu_k[i+1] - cu_k[i]) of
 // (slots[i], seqs[i]) into rows cu_k[i].. of k_pack / v_pack (total rows each).
-// Block (chunk stride, segment, K or V).
+// Block (chunk stride, segment, part of the row of K or V).
 template <typename T>
 __global__ void __launch_bounds__(kQ8Threads)
     q8_gather_kernel(const Q8Cache c, T* k_pack, T* v_pack, const int32_t* slots, const int32_t* seqs,
-                     const int32_t* cu_k, long long total, int* err) {
+                     const int32_t* cu_k, long long total, int log2_dh, int* err) {
   griddep_wait();
-  extern __shared__ int8_t s_exp[];
+  __shared__ int8_t s_exp[kQ8Heads][kQ8Chunk];
   const int i = blockIdx.y;
-  const bool isv = blockIdx.z != 0;
+  const bool isv = (blockIdx.z & 1) != 0;
   const int slot = slots[i], seq = seqs[i];
   const long long k0 = cu_k[i], len = (long long)cu_k[i + 1] - k0;
   const bool ok_slot = slot >= 0 && slot < c.n_slots && seq >= 0 && seq < c.n_seqs;
   if (!ok_slot || len < 0 || len > c.max_seq || k0 < 0 || k0 + len > total) {
-    if (threadIdx.x == 0 && blockIdx.x == 0 && !isv) set_error(err, ok_slot ? kErrBadPos : kErrBadSlot);
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.z == 0) set_error(err, ok_slot ? kErrBadPos : kErrBadSlot);
     return;
   }
-  const int lanes = c.Dh >> 3, width = c.Hkv * c.Dh;
-  const int8_t* esrc = (isv ? c.ve : c.ke) + c.exps(slot, seq);
+  const int width = c.Hkv * c.Dh;
+  const int x0 = (blockIdx.z >> 1) * kQ8Span;
+  constexpr int PER = kQ8Span / 8, STEP = kQ8Threads / PER, U = kQ8Chunk / STEP;
+  const int xi = (threadIdx.x % PER) * 8, x = x0 + xi, j0 = threadIdx.x / PER;
+  const bool on = x < width;
+  const int h0 = x0 >> log2_dh, nh = min(kQ8Span, width - x0) >> log2_dh;
+  const int8_t* esrc = (isv ? c.ve : c.ke) + c.exps(slot, seq) + (long long)h0 * c.max_seq;
   for (long long p0 = (long long)blockIdx.x * kQ8Chunk; p0 < len; p0 += (long long)gridDim.x * kQ8Chunk) {
     const int np = (int)min((long long)kQ8Chunk, len - p0);
+    const uint8_t* src = (isv ? c.v : c.k) + c.row(slot, seq, (int)p0) + x;
+    T* dst = (isv ? v_pack : k_pack) + (k0 + p0) * width + x;
+    uint2 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * STEP;
+      q[u] = on && j < np ? *reinterpret_cast<const uint2*>(src + (long long)j * width) : make_uint2(0, 0);
+    }
     __syncthreads();  // the previous chunk's exponents are read
-    for (int t = threadIdx.x; t < c.Hkv * kQ8Chunk; t += kQ8Threads) {
+    for (int t = threadIdx.x; t < nh * kQ8Chunk; t += kQ8Threads) {
       const int h = t / kQ8Chunk, j = t % kQ8Chunk;
-      if (j < np) s_exp[t] = esrc[(long long)h * c.max_seq + p0 + j];
+      if (j < np) s_exp[h][j] = esrc[(long long)h * c.max_seq + p0 + j];
     }
     __syncthreads();
-    const uint8_t* src = (isv ? c.v : c.k) + c.row(slot, seq, (int)p0);
-    T* dst = (isv ? v_pack : k_pack) + (k0 + p0) * width;
-    const int units = np * c.Hkv * lanes;
-    constexpr int U = 4;
-    for (int e0 = 0; e0 < units; e0 += U * kQ8Threads) {
-      uint2 q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int e = e0 + u * kQ8Threads + threadIdx.x;
-        q[u] = e < units ? *reinterpret_cast<const uint2*>(src + (long long)e * 8) : make_uint2(0, 0);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int e = e0 + u * kQ8Threads + threadIdx.x;
-        if (e < units) {
-          const int hr = e / lanes;
-          const float s = exp2_int(s_exp[(hr % c.Hkv) * kQ8Chunk + hr / c.Hkv]);
-          float a[4], b[4];
-          e4m3x4_to_f(q[u].x, a);
-          e4m3x4_to_f(q[u].y, b);
-          const float f[8] = {a[0] * s, a[1] * s, a[2] * s, a[3] * s, b[0] * s, b[1] * s, b[2] * s, b[3] * s};
-          Vec8<T>::store(dst + (long long)e * 8, f);
-        }
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * STEP;
+      if (on && j < np) {
+        const float s = exp2_int(s_exp[xi >> log2_dh][j]);
+        float a[4], b[4];
+        e4m3x4_to_f(q[u].x, a);
+        e4m3x4_to_f(q[u].y, b);
+        const float f[8] = {a[0] * s, a[1] * s, a[2] * s, a[3] * s, b[0] * s, b[1] * s, b[2] * s, b[3] * s};
+        Vec8<T>::store(dst + (long long)j * width, f);
       }
     }
   }

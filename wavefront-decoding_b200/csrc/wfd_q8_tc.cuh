@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
     constexpr uint32_t IDESC_PV = q8_idesc(N, true, true);
     const uint32_t q_addr = smem_u32(qs), p_addr = smem_u32(ps), k_addr = smem_u32(kts), v_addr = smem_u32(vts);
     const uint32_t tm = uniform(tmem);
-    uint32_t ks = 0, vs = 0, kp = 0;   // of S's step
+    uint32_t ks = 0, kp = 0;           // of S's step
     uint32_t pv = 0, pvs = 0, pvp = 0; // P.V issued so far, its V slot and phase
     uint32_t two_tiles = 0;            // of the steps pv, pv + 1, ..: whether they have a second tile
     // P.V of the next step, if its weights and its V tiles are there (last: waits)

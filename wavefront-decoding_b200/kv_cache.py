@@ -324,7 +324,13 @@ class QuantKVCache(SlotKVCache):
 
     def wave_attn(self, q, k_new, v_new, items, max_q: int, *, slot_offset: int = 0, out=None, kernel: int = -1,
                   update_lens: bool = True, row_pos=None):
-        """Fused quantising append + wavefront attention over this cache's slots."""
-        return _attn.wave_attn_q8(q, k_new, v_new, self.K, self.V, self.k_exp, self.v_exp, items, max_q,
-                                  lens=self.lens if update_lens else None, slot_offset=slot_offset, out=out,
-                                  kernel=kernel, row_pos=row_pos)
+        """Fused quantising append + wavefront attention over this cache's slots (attention.wave_attn_q8)."""
+        if not update_lens:
+            return _attn.wave_attn_q8(q, k_new, v_new, self.K, self.V, self.k_exp, self.v_exp, items, max_q,
+                                      slot_offset=slot_offset, out=out, kernel=kernel, row_pos=row_pos)
+        if rt.require_cuda(q) != self.device:
+            raise ValueError(f"rows on {q.device}, cache on {self.device}")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        _ops.wave_attn_q8_launch(self._c, q, k_new, v_new, items, int(max_q), int(slot_offset), None, int(kernel),
+                                 row_pos, out)
+        return out

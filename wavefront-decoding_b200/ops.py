@@ -39,6 +39,7 @@ dispatcher.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -139,6 +140,11 @@ def _check_commit(k_cache, v_cache, lens, items, accept_len, accept_mask):
     if accept_mask is not None and accept_mask.dtype != torch.uint8:
         raise ValueError("accept_mask must be uint8")
     return dev
+
+
+def plain_eager(t: torch.Tensor) -> bool:
+    """Whether a call on t can go to the kernel without the dispatcher: a plain tensor, nothing compiling or tracing."""
+    return type(t) is torch.Tensor and torch._C._len_torch_dispatch_stack() == 0 and not torch.compiler.is_compiling()
 
 
 def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
@@ -256,9 +262,15 @@ def _commit_drop_cuda(lens, drop_pos):
 
 def _wave_attn_q8_out_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens, slot_offset, scale,
                            kernel, row_pos, out):
-    dev = rt.require_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, lens, row_pos, out)
-    c = q8_cache_struct(k_cache, v_cache, k_exp, v_exp, lens)
-    Hkv, Dh = k_cache.shape[3:]
+    rt.require_cuda(q, k_cache, v_cache, k_exp, v_exp, lens)
+    wave_attn_q8_launch(q8_cache_struct(k_cache, v_cache, k_exp, v_exp, lens), q, k_new, v_new, items, max_q,
+                        slot_offset, scale, kernel, row_pos, out)
+
+
+def wave_attn_q8_launch(c, q, k_new, v_new, items, max_q, slot_offset, scale, kernel, row_pos, out) -> None:
+    """wfd_wave_attn_q8 over the cache struct c (on q's device), after the checks of the other arguments."""
+    dev = rt.require_cuda(q, k_new, v_new, items, row_pos, out)
+    Hkv, Dh = c.n_kv_heads, c.head_dim
     if q.dim() != 3 or q.shape[2] != Dh or k_new.shape != (q.shape[0], Hkv, Dh) or v_new.shape != k_new.shape:
         raise ValueError("q (n_rows, H, Dh) and k_new / v_new (n_rows, Hkv, Dh) must match the cache")
     if q.dtype != k_new.dtype or q.dtype != v_new.dtype:
@@ -287,6 +299,7 @@ def _wave_attn_q8_out_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, item
             rt.error_word(dev).data_ptr(), rt.stream_ptr(dev))
 
 
+@functools.lru_cache(maxsize=4096)
 def q8_workspace_bytes(dev: torch.device, n: int) -> int:
     with torch.cuda.device(dev):
         b = int(_abi.load().wfd_wave_attn_q8_workspace(n))
