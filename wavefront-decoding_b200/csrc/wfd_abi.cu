@@ -1661,8 +1661,8 @@ int launch_sample(const SampleParams& p, int cluster, size_t smem, cudaStream_t 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WFD_ERR_CUDA;
   if (!attr_set[dev].load()) {
-    constexpr int most = (int)sizeof(SampleShared) + kSampleMaxV / 256 * 8;
-    if (cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+    if (cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleSmem) !=
+        cudaSuccess)
       return WFD_ERR_CUDA;
     attr_set[dev].store(true);
   }
@@ -1720,11 +1720,20 @@ extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
   p.u_cols = a->u_cols;
   p.seq_stride = a->seq_stride;
   p.pos_stride = a->pos_stride;
-  // CTAs per row: as many as fit at two CTAs an SM, with at least a tile of tokens each
+  // CTAs per row: as many as fit at two CTAs an SM, with at least a tile of tokens
+  // each; and more, up to 8, where that lets a slice fit in half an SM's shared memory
   int cluster = 1;
-  while (cluster < 8 && (long long)a->n * cluster * 2 <= 2ll * sms && cluster * kSampleTile < a->V) cluster *= 2;
-  p.slice = ((a->V + cluster - 1) / cluster + kSampleTile - 1) / kSampleTile * kSampleTile;
-  const size_t smem = sizeof(SampleShared) + (size_t)p.slice / 256 * 8;
+  auto slice_of = [&](int c) { return ((a->V + c - 1) / c + kSampleTile - 1) / kSampleTile * kSampleTile; };
+  auto smem_of = [&](int c, bool cached) {
+    const size_t n = (size_t)slice_of(c);
+    return sizeof(SampleShared) + n / 256 * 8 + (cached ? n * eb : 0);
+  };
+  while (cluster < 8 && cluster * kSampleTile < a->V &&
+         ((long long)a->n * cluster * 2 <= 2ll * sms || smem_of(cluster, true) > kSampleSmem))
+    cluster *= 2;
+  p.slice = slice_of(cluster);
+  p.cached = smem_of(cluster, true) <= kSampleSmem ? 1 : 0;
+  const size_t smem = smem_of(cluster, p.cached != 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return a->dtype == WFD_DTYPE_BF16 ? launch_sample<__nv_bfloat16>(p, cluster, smem, st)
                                     : launch_sample<float>(p, cluster, smem, st);

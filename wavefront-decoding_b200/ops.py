@@ -91,6 +91,8 @@ def heads(q: torch.Tensor, k: torch.Tensor) -> tuple[int, int, int]:
 
 
 def i32(t, device) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
     t = torch.as_tensor(t)
     if t.dtype != torch.int32 or t.device != device:
         t = t.to(device=device, dtype=torch.int32)
