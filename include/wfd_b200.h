@@ -321,8 +321,9 @@ int wfd_commit_window_q8(const wfd_q8_cache* cache, const wfd_item* items, int32
 /* wfd_wave_attn over an 8-bit cache: the window rows are quantised into the
  * cache, then every row attends the values the cache holds, its own included.
  * q / out and k_new / v_new are `dtype` (bf16 or f32); head_dim 64 or 128; max_q an
- * upper bound of the items' q_len (a longer item is reported).  row_pos as in
- * wfd_wave_attn_rows, for either kernel.  which: -1 auto, 0 CUDA cores, 1 tcgen05
+ * upper bound of the items' q_len (what the tcgen05 kernel cannot hold of a longer
+ * item is not computed, and reported).  row_pos as in wfd_wave_attn_rows, for
+ * either kernel.  which: -1 auto, 0 CUDA cores, 1 tcgen05
  * (bf16; n_kv_heads * head_dim a multiple of 128).  scale 0 selects
  * 1/sqrt(head_dim); a negative one is refused.  Where two items hold one position of a
  * (slot, sequence), the later item's row is stored.  The workspace

@@ -412,6 +412,22 @@ def test_attn_scale_and_bad_items(cuda_dev):
         assert torch.equal(c2.K.view(torch.uint8), before) and (res == 7).all() and (c2.lens == 0).all()
 
 
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_attn_item_longer_than_max_q(cuda_dev, kernel):
+    """Either computed or, where the kernel's variant has no room, reported and its rows left; the cache is written."""
+    items = [(0, 0, 130, 5, 0), (1, 1, 64, 1, 5)]
+    out, c, o = run_attn(cuda_dev, H=8, items=items, max_q=1, kernel=kernel, check=False)
+    if kernel:
+        assert error_bits(cuda_dev) == 8
+    else:
+        no_error(cuda_dev)
+    same_cache(c, o)
+    ref, _, _ = run_attn(cuda_dev, H=8, items=items, kernel=kernel)
+    # the item within max_q: two results, each off by 2^-8 in its weights and 2^-8 in its rounding (2^-10 for the rest)
+    vmax = np.abs(o.values(1, 1, 65)[1]).max()
+    assert np.abs(f64(out[5]) - f64(ref[5])).max() <= 2 * (2.0 ** -7 + 2.0 ** -10) * vmax
+
+
 def test_attn_repeats_bit_for_bit_and_captures(cuda_dev):
     """The same call twice, and a captured one replayed with new positions."""
     from wavefront_decoding_b200 import attention as wa

@@ -120,6 +120,15 @@ def test_borders_of_the_parameters(cuda_dev):
         check(cuda_dev, x, u, k=10, p=0.8)
 
 
+@pytest.mark.parametrize("spread,T", [(1e37, 1e37), (8e37, 2e38), (1e38, float("inf")), (3.0, 1e30), (1e-38, 1e-40)])
+def test_distances_and_temperatures_at_the_type_s_ends(cuda_dev, spread, T):
+    """m0 - x, or the range of the histogram, past fp32's largest value; temperatures below its normal ones."""
+    x, r = logits(11, 12, 9000, "f32", spread)
+    x.clamp_(-3.4e38, 3.4e38)
+    check(cuda_dev, x, r[0], T=T, p=0.05 + 0.9 * r[1])
+    check(cuda_dev, x, r[0], T=T, k=(1 + r[2] * 8000).int(), p=0.05 + 0.9 * r[1], m=0.5 * r[3])
+
+
 def test_shares_of_many_draws(cuda_dev):
     """u on a fine grid reproduces the probabilities: the share of each id is its weight to within one grid step."""
     from wavefront_decoding_b200 import fused

@@ -1412,7 +1412,7 @@ int launch_q8_cols(long long nv, const Q8AttnParams& ap, const Q8Maps& maps, int
 
 template <typename T, int DH>
 int launch_q8_simt(int nq, const Q8AttnParams& ap, int sms, cudaStream_t st) {
-  const dim3 g(sms), b(kQ8SimtThreads);
+  const dim3 g(sms), b(q8_simt_threads(nq));
   cudaError_t e = nq == 1   ? launch_pdl(q8_attn_kernel<T, DH, 1>, g, b, 0, st, ap)
                   : nq == 2 ? launch_pdl(q8_attn_kernel<T, DH, 2>, g, b, 0, st, ap)
                             : launch_pdl(q8_attn_kernel<T, DH, 4>, g, b, 0, st, ap);

@@ -31,15 +31,16 @@ struct Q8AttnParams : VerifyParams {
 // one more to merge.
 constexpr int kQ8MinShare = 256;
 
-constexpr int kQ8SimtThreads = 384;
+// Threads of a CTA, one CTA an SM: 4 vectors' queries and sums take 128 registers.
+__host__ __device__ constexpr int q8_simt_threads(int nq) { return nq == 4 ? 256 : 384; }
 constexpr int kQ8SimtNQ = 4;  // query vectors per unit, at most
 
 template <typename T, int DH, int NQ>
-__global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8AttnParams p) {
+__global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q8AttnParams p) {
   constexpr int LPR = DH / 16;      // lanes per key row
   constexpr int KPW = 32 / LPR;     // keys per warp step
   constexpr int U = 4;              // steps in flight
-  constexpr int WARPS = kQ8SimtThreads / 32;
+  constexpr int THREADS = q8_simt_threads(NQ), WARPS = THREADS / 32;
   const float NEG_INF = -__int_as_float(0x7f800000);
   __shared__ float s_q[NQ][DH];
   __shared__ int s_lim[NQ];               // last key a vector sees
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8Attn
       return ((long long)(S.q_row0 + v / p.G) * p.Hq + h * p.G + v % p.G) * DH;
     };
     __syncthreads();  // the previous unit's shared state is read
-    for (int i = tid; i < NQ * DH; i += kQ8SimtThreads) {
+    for (int i = tid; i < NQ * DH; i += THREADS) {
       const int n = i / DH;
       s_q[n][i % DH] = n < nvec ? to_f<T>(q[q_at(n) + i % DH]) : 0.f;
     }
@@ -108,18 +109,19 @@ __global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8Attn
     for (int kb = r_lo + warp * (KPW * U); kb < r_hi; kb += WARPS * KPW * U) {
       uint4 kq[U], vq[U];
       float ks[U], vs[U];
+      signed char ke[U], ve[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {  // loads without branches: all in flight at once
+        const int key = min(kb + j * KPW + grp, r_hi - 1);
+        kq[j] = *reinterpret_cast<const uint4*>(p.c.k + c0 + key * row_codes);
+        vq[j] = *reinterpret_cast<const uint4*>(p.c.v + c0 + key * row_codes);
+        ke[j] = p.c.ke[e0 + key];
+        ve[j] = p.c.ve[e0 + key];
+      }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int key = kb + j * KPW + grp;
-        const bool on = key < r_hi;
-        kq[j] = vq[j] = make_uint4(0, 0, 0, 0);
-        ks[j] = vs[j] = 0.f;
-        if (on) {
-          kq[j] = *reinterpret_cast<const uint4*>(p.c.k + c0 + key * row_codes);
-          vq[j] = *reinterpret_cast<const uint4*>(p.c.v + c0 + key * row_codes);
-          ks[j] = exp2_int(p.c.ke[e0 + key]);
-          vs[j] = exp2_int(p.c.ve[e0 + key]);
-        }
+        ks[j] = exp2_int(ke[j]);
+        vs[j] = exp2_int(ve[j]);
       }
       float s[U][NQ];
 #pragma unroll
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8Attn
     const int c_last = (int)((ustart + S.k_len - 1) / share);
     const int n_contrib = p.invariant ? 1 : c_last - c_first + 1;
     constexpr int PART = NQ * (DH + 2);
-    for (int i = tid; i < nvec * DH; i += kQ8SimtThreads) {
+    for (int i = tid; i < nvec * DH; i += THREADS) {
       const int n = i / DH, d = i % DH;
       float M = NEG_INF;
 #pragma unroll
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(kQ8SimtThreads, 1) q8_attn_kernel(const Q8Attn
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int i = tid; i < nvec * DH; i += kQ8SimtThreads) {
+        for (int i = tid; i < nvec * DH; i += THREADS) {
           const int n = i / DH, d = i % DH;
           float M = NEG_INF, L = 0.f, O = 0.f;
           for (int k = 0; k < n_contrib; ++k) {  // in key order, whoever arrives last
