@@ -15,6 +15,11 @@
 // Every lane group keeps its own running (m, l, O); groups, warps and CTAs are
 // merged at the end of a unit.  Up to 4 query vectors per unit: q and O take 128
 // registers; more vectors are further units over the same keys.
+//
+// Bound by latency: 32 windows of 3 rows over 777 keys, 8 heads of 64, fp32, take
+// 28 us (4 us of HBM time), three units a CTA of three rounds of 256 keys, each
+// waiting for its loads, and a merge of 8 warps.  (Loads in branches, one round trip
+// each, and 12 warps that spilled: 41 us; scalar products instead of pairs: 30.)
 #pragma once
 
 #include "wfd_q8.cuh"
@@ -26,10 +31,33 @@ struct Q8AttnParams : VerifyParams {
   Q8Cache c;  // counted from the call's slot offset
 };
 
-// A CTA's share is at least this many keys of one unit: a piece of fewer takes as
-// long as a whole tile pair of the tensor-core kernel, and every further piece is
-// one more to merge.
+// A CTA's share is at least this many keys of one unit, a round of its 8 to 12 warps:
+// a piece of fewer takes as long, and every further piece is one more to merge.
 constexpr int kQ8MinShare = 256;
+
+// Two fp32 values in one 64-bit register: one instruction for both.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void up2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 // Threads of a CTA, one CTA an SM: 4 vectors' queries and sums take 128 registers.
 __host__ __device__ constexpr int q8_simt_threads(int nq) { return nq == 4 ? 256 : 384; }
@@ -90,14 +118,15 @@ __global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q
                                           : S.k_len - S.q_len + row;
     }
     __syncthreads();
-    float qr[NQ][16], acc[NQ][16], m[NQ], l[NQ];
+    f32x2 qr[NQ][8], acc[NQ][8];
+    float m[NQ], l[NQ];
     int lim[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        qr[n][i] = s_q[n][sub * 16 + i];
-        acc[n][i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        qr[n][i] = pk2(s_q[n][sub * 16 + 2 * i], s_q[n][sub * 16 + 2 * i + 1]);
+        acc[n][i] = pk2(0.f, 0.f);
       }
       m[n] = NEG_INF;
       l[n] = 0.f;
@@ -126,20 +155,23 @@ __global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q
       float s[U][NQ];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
+        f32x2 s2[NQ];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) s[j][n] = 0.f;
+        for (int n = 0; n < NQ; ++n) s2[n] = pk2(0.f, 0.f);
         const uint32_t w[4] = {kq[j].x, kq[j].y, kq[j].z, kq[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float f[4];
           e4m3x4_to_f(w[i], f);
+          const f32x2 f0 = pk2(f[0], f[1]), f1 = pk2(f[2], f[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) s[j][n] = fmaf(qr[n][4 * i + e], f[e], s[j][n]);
+          for (int n = 0; n < NQ; ++n) s2[n] = fma2(qr[n][2 * i + 1], f1, fma2(qr[n][2 * i], f0, s2[n]));
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
+          float s_even, s_odd;
+          up2(s2[n], s_even, s_odd);
+          s[j][n] = s_even + s_odd;
 #pragma unroll
           for (int o = LPR / 2; o > 0; o >>= 1) s[j][n] += __shfl_xor_sync(0xffffffffu, s[j][n], o);
           const int key = kb + j * KPW + grp;
@@ -156,7 +188,7 @@ __global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q
         m[n] = mn;
         l[n] *= cr;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][i] *= cr;
+        for (int i = 0; i < 8; ++i) acc[n][i] = mul2(acc[n][i], pk2(cr, cr));
 #pragma unroll
         for (int j = 0; j < U; ++j) {
           const float w = fast_exp2((s[j][n] - ms) * c2);
@@ -171,10 +203,13 @@ __global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q
         for (int i = 0; i < 4; ++i) {
           float f[4];
           e4m3x4_to_f(w[i], f);
+          const f32x2 f0 = pk2(f[0], f[1]), f1 = pk2(f[2], f[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) acc[n][4 * i + e] = fmaf(s[j][n], f[e], acc[n][4 * i + e]);
+          for (int n = 0; n < NQ; ++n) {
+            const f32x2 wn = pk2(s[j][n], s[j][n]);
+            acc[n][2 * i] = fma2(wn, f0, acc[n][2 * i]);
+            acc[n][2 * i + 1] = fma2(wn, f1, acc[n][2 * i + 1]);
+          }
         }
       }
     }
@@ -190,15 +225,15 @@ __global__ void __launch_bounds__(q8_simt_threads(NQ), 1) q8_attn_kernel(const Q
         const float ca = fast_exp2((m[n] - ms) * c2), cb = fast_exp2((mo - ms) * c2);
         l[n] = l[n] * ca + lo * cb;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float ao = __shfl_xor_sync(0xffffffffu, acc[n][i], o);
-          acc[n][i] = acc[n][i] * ca + ao * cb;
+        for (int i = 0; i < 8; ++i) {
+          const f32x2 ao = __shfl_xor_sync(0xffffffffu, acc[n][i], o);
+          acc[n][i] = fma2(ao, pk2(cb, cb), mul2(acc[n][i], pk2(ca, ca)));
         }
         m[n] = mn;
       }
       if (grp == 0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_o[warp][n][sub * 16 + i] = acc[n][i];
+        for (int i = 0; i < 8; ++i) up2(acc[n][i], s_o[warp][n][sub * 16 + 2 * i], s_o[warp][n][sub * 16 + 2 * i + 1]);
         if (sub == 0) {
           s_m[warp][n] = m[n];
           s_l[warp][n] = l[n];
