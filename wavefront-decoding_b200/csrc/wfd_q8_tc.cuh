@@ -779,12 +779,15 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
       int arrived = 0;
       // (the plan kernel clears the counters, so they are read after it only)
       if (n_contrib > 1 && stid == 0 && s.waited) arrived = ld_relaxed_gpu(p.ws_cnt + c_first);
+      int frontier = S.k_len - S.q_len;  // the first row's position: keys up to it need no mask
       if (p.row_pos != nullptr) {
         if (sq == 0 && lane < NL) {
           const int n = col0 + lane;
           sh.rp[n] = n < nvec ? p.row_pos[(long long)(S.q_row0 + uc.vec(n) / p.G) * p.row_pos_stride] : -1;
         }
         softmax_bar<SMT>();
+        // of these columns, the first row's position
+        frontier = __reduce_min_sync(0xffffffffu, lane < NL && col0 + lane < nvec ? sh.rp[col0 + lane] : 0x7fffffff);
       }
       q8_wait(&sh.qready[s.unit & 3u], (s.unit >> 2) & 1u, abort_flag, p.err);
       const float* csc = sh.cscale[s.unit & 3u] + col0;
@@ -853,7 +856,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
         // masking, as K2: nothing to do on a step inside the unit and below the causal
         // frontier of the window's first row
         const int last = k0 + STEP - 1;
-        if (last >= r_hi || col0 + NL > nvec || p.row_pos != nullptr || last > S.k_len - S.q_len) {
+        if (last >= r_hi || col0 + NL > nvec || last > frontier) {
 #pragma unroll
           for (int hf = 0; hf < T; ++hf) {
             const int key = k0 + hf * kTcTile + my_row;
