@@ -81,7 +81,7 @@ class LoopedLMConfig:
         return 2 * self.vocab * d + d + (self.n_prelude + self.n_core + self.n_coda) * per_layer
 
 
-# the configurations BASELINE.json names
+# the named configurations
 CONFIG1 = LoopedLMConfig()  # vocab 32000, d 512, 8 x 64, SwiGLU 1536, prelude 1 / core 2 x R=4 / coda 1
 CONFIG4 = LoopedLMConfig(vocab=50304, d_model=1536, n_heads=24, n_kv_heads=24, head_dim=64, d_ff=4096,
                          n_prelude=2, n_core=4, n_coda=2, T_total=8)
