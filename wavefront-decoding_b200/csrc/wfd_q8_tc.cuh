@@ -9,21 +9,29 @@
 // columns n and NQP + n of the same MMA:
 //     x 2^-e = x1 + x2 / 16,  x1 = e4m3(x 2^-e),  x2 = e4m3(16 (x 2^-e - x1))
 // (e from the row's largest element, |x 2^-e| <= 448, so |16 (.. - x1)| <= 256).
-//   Q: a bf16 value has 8 significant bits, so both pieces together are exact down
-//      to 2^-23 of the row's largest element.
+//   Q: a bf16 value has 8 significant bits, so both pieces together are exact until
+//      the low one underflows: off by at most 2^-14 where the row's largest element
+//      is 224 to 448, 2^-21.8 of it.
 //   P: each piece is off by at most half a step, 2^-4 of its value: 2^-8 together,
-//      what rounding P to bf16 costs, down to weights of 2^-16 of the largest (an
-//      attention sink over 64k flat keys stays inside that).  The weights' sum is
-//      taken of the unrounded weights in fp32.
+//      what rounding P to bf16 costs.  A step's weights are scaled by that step's own
+//      largest, 2^8 there, and O of the step joins the unit's in fp32
+//      under 2^(step's maximum - M): where the low piece underflows, below 2^-14 of
+//      the step's largest weight, a weight is off by at most 2^-22 of it, so the
+//      256 keys of a step lose 2^-14 of it together, however many steps there are.
+//      (Scaled by the running maximum instead, weights below 2^-22 of it were zero:
+//      one key 15 nats above a flat prefix hid all of the rest.)  The weights' sum
+//      is taken of the unrounded weights in fp32.
 // The minimum N of the instruction leaves room for the second piece, so a tile of
 // 32 KB takes 8 MMAs, half of the bf16 kernel's for the same bytes.
 //     S^T[128 keys x 2 NQP] = K . [Q1 | Q2]^T         (K-major, 4 k-steps of 32 bytes)
 //     O^T[128 dims x 2 NQP] += V^T . [P1 | P2]^T       (both MN-major, 4 k-steps of 32 keys)
 // Scales: a key's 2^{e_k} multiplies its finished score; its value scale joins the
-// weight, t = s + e_v in log2 units, so that the running maximum is taken of t and
-// the weights stay within e4m3's range: w = 2^(t - M + 8), M moved when a tile
-// exceeds it by 3/4 (w <= 431 < 448).  The denominator needs 2^(s - M + 8) = w 2^{-e_v}.
-// |e_v| <= 32 keeps that above the fp32 underflow for every key that matters.
+// weight, t = s + e_v in log2 units, so that the maxima are taken of t and the
+// weights stay within e4m3's range: w = 2^(t - m + 8) <= 2^8, m the step's maximum.
+// Sums are held relative to M, a maximum that moves only when a step's exceeds it by
+// 16: what it leaves, w 2^(m - M) |code| <= 2^33 a key, is far inside fp32.  The
+// denominator needs 2^(s - M + 8) = w 2^{-e_v} 2^(m - M); |e_v| <= 32 keeps that above
+// the fp32 underflow for every key that matters.
 //
 // What bounds it: HBM; a step of 256 keys (64 KB of K and V) takes 1.5 us of an SM's
 // share of the copy bandwidth.  Behind it come two chains:
@@ -323,6 +331,12 @@ __device__ __forceinline__ void self_start(const VerifyParams& p, SelfStart& sh,
   __syncthreads();
 }
 
+// Per softmax warp and column, of a step: what the exponents add, the factor of what
+// the unit holds (1 unless M moved), the factor 2^(m - M) of what the step adds (of
+// the last two steps: O joins one step late).
+enum : int { kMxSub = 0, kMxMove = 16, kMxStep = 32 };
+constexpr float kQ8Lead = 16.f;  // how far a step's maximum may exceed M
+
 // Shared memory besides the tiles.
 template <typename C, int NQP>
 struct Q8Shared {
@@ -330,7 +344,7 @@ struct Q8Shared {
   float red[2][4][NQP];                  // column maxima of each warp
   float lred[2][4][NQP];                 // column sums
   float cscale[4][NQP];                  // score scale of each column, per unit
-  float mx[C::WARPS][2][16];             // per softmax warp: what the exponentials subtract, rescale factors
+  float mx[C::WARPS][4][16];             // per softmax warp: kMxSub, kMxMove, kMxStep (two steps')
   uint64_t kfull[C::KS], vfull[C::VS], vempty[C::VS];
   uint64_t sfull[C::KS], sfree[C::KS];   // S of a step complete (its K free), and read by the softmax
   uint64_t pfull, ofull;                 // P written (so the O of the step before is read), P.V complete
@@ -791,14 +805,14 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
       }
       q8_wait(&sh.qready[s.unit & 3u], (s.unit >> 2) & 1u, abort_flag, p.err);
       const float* csc = sh.cscale[s.unit & 3u] + col0;
-      // The running maximum of column col0 + j (j < NL) lives in lane j of every
-      // softmax warp of the slice: what the exponentials subtract (8 below it) and the
-      // step's rescale factors reach the other lanes through shared memory.
+      // M of column col0 + j (j < NL) lives in lane j of every softmax warp of the
+      // slice; a step's factors reach the other lanes through shared memory.
       float m = NEG_INF;
       f32x2 lp[NP], oacc[NP];
 #pragma unroll
       for (int j = 0; j < NP; ++j) lp[j] = oacc[j] = 0ull;
-      auto add_o = [&](uint32_t i) {  // P.V of step i joins O
+      auto add_o = [&](uint32_t i, int t) {  // P.V of step i, the unit's t, joins O
+        const float* ms = mw + kMxStep + 16 * (t & 1);
         q8_wait(&sh.ofull, i & 1u, abort_flag, p.err);
         tc_fence_after();
         float o0[NL], o1[NL];
@@ -807,8 +821,10 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
         tc_wait_ld();
         tc_fence_before();
 #pragma unroll
-        for (int j = 0; j < NP; ++j)
-          oacc[j] = add2(oacc[j], fma2(pk2(o1[2 * j], o1[2 * j + 1]), c16, pk2(o0[2 * j], o0[2 * j + 1])));
+        for (int j = 0; j < NP; ++j) {
+          const float2 sj = *reinterpret_cast<const float2*>(ms + 2 * j);
+          oacc[j] = fma2(fma2(pk2(o1[2 * j], o1[2 * j + 1]), c16, pk2(o0[2 * j], o0[2 * j + 1])), pk2(sj.x, sj.y), oacc[j]);
+        }
       };
       // a per-head pair of values for the columns (2 j, 2 j + 1)
       auto by_head = [&](int j, float v0, float v1) {
@@ -892,24 +908,28 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
           if (lane == 0) *reinterpret_cast<float2*>(rb + sq * NQP + col0 + 2 * j) = make_float2(m0, m1);
         }
         softmax_bar<SMT>();
-        if (t >= 1) add_o(i - 1);  // relative to the maximum before this step; also frees P^T
+        if (t >= 1) add_o(i - 1, t - 1);  // relative to M before this step; also frees P^T
         float al = 1.f;
         if (lane < NL) {
           const int c = col0 + lane;
           const float mx = fmaxf(fmaxf(rb[c], rb[NQP + c]), fmaxf(rb[2 * NQP + c], rb[3 * NQP + c]));
-          if (mx > m + 0.75f) {
-            al = ex2_ftz(m - mx);
-            m = mx;
+          const bool none = mx == NEG_INF;  // no key seen: exp2(-inf) = 0
+          const float sub = none ? 0.f : 8.f - mx;
+          const float ms = 8.f - sub;  // the maximum that `sub` stands for: its rounding enters no ratio of steps
+          if (!none && ms > m + kQ8Lead) {
+            al = ex2_ftz(m - ms);
+            m = ms;
           }
-          mw[lane] = m == NEG_INF ? 0.f : 8.f - m;  // no key seen: exp2(-inf) = 0
-          mw[16 + lane] = al;
+          mw[kMxSub + lane] = sub;
+          mw[kMxMove + lane] = al;
+          mw[kMxStep + 16 * (t & 1) + lane] = none ? 0.f : ex2_ftz(ms - m);
         }
         const bool moved = __any_sync(0xffffffffu, al != 1.f);
         __syncwarp();
         if (moved) {
 #pragma unroll
           for (int j = 0; j < NP; ++j) {
-            const float2 aj = *reinterpret_cast<const float2*>(mw + 16 + 2 * j);
+            const float2 aj = *reinterpret_cast<const float2*>(mw + kMxMove + 2 * j);
             lp[j] = mul2(lp[j], pk2(aj.x, aj.y));
             oacc[j] = mul2(oacc[j], pk2(aj.x, aj.y));
           }
@@ -926,19 +946,21 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
             }
           }
         }
-        // weights 2^(t - M + 8); the denominator's leave the value scale out again.
+        // weights 2^(t - m + 8); the denominator's leave the value scale out again.
         // (A step of one tile: the other's are zero, and no MMA reads them.)
         uint32_t w1[T][(NL + 3) / 4], w2[T][(NL + 3) / 4];
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          const float2 mj = *reinterpret_cast<const float2*>(mw + 2 * j);
+          const float2 mj = *reinterpret_cast<const float2*>(mw + kMxSub + 2 * j);
+          const float2 sj = *reinterpret_cast<const float2*>(mw + kMxStep + 16 * (t & 1) + 2 * j);
+          f32x2 ls = 0ull;  // the step's sum
 #pragma unroll
           for (int hf = 0; hf < T; ++hf) {
             const float ia = exp2_int(-(int)(signed char)(ew[hf] >> 8)), ib = exp2_int(-(int)(signed char)(ew[hf] >> 24));
             float d0, d1;
             up2(add2(x[hf][j], pk2(mj.x, mj.y)), d0, d1);
             const f32x2 w = pk2(ex2_ftz(d0), ex2_ftz(d1));
-            lp[j] = fma2(w, by_head(j, ia, ib), lp[j]);
+            ls = fma2(w, by_head(j, ia, ib), ls);
             uint32_t p1, p2;
             q8_split(w, p1, p2);
             if ((j & 1) == 0) {
@@ -949,6 +971,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
               w2[hf][j / 2] |= p2 << 16;
             }
           }
+          lp[j] = fma2(ls, pk2(sj.x, sj.y), lp[j]);
         }
 #pragma unroll
         for (int hf = 0; hf < T; ++hf) {
@@ -972,7 +995,7 @@ __global__ void __launch_bounds__(q8_tc_threads(NA), q8_ctas(NA))
         softmax_bar<SMT>();
         if (stid == 0) mbar_arrive(&sh.pfull);
       }
-      add_o(s.step + (uint32_t)n_t - 1);
+      add_o(s.step + (uint32_t)n_t - 1, n_t - 1);
 
       // ---- column sums of the weights over the unit's keys
       float* lb = sh.lred[s.unit & 1u][0];
