@@ -224,6 +224,7 @@ class QuantKVCache(SlotKVCache):
         return self.K.numel() + self.V.numel() + self.k_exp.numel() + self.v_exp.numel()
 
     def _call(self, name: str, *args) -> None:
+        rt.require_cuda(self.K)
         rt.call(self.device, name, ctypes.byref(self._c), *args, rt.error_word(self.device).data_ptr(),
                 self._stream())
 

@@ -150,7 +150,7 @@ def plain_eager(t: torch.Tensor) -> bool:
 
 
 def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
-    """The C view of an 8-bit cache's tensors, after the checks of their shapes and types."""
+    """The C view of an 8-bit cache's tensors, after the checks of their shapes, types and devices."""
     if k.dim() != 5 or v.shape != k.shape or k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or \
             not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("K, V must be contiguous float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) tensors")
@@ -162,6 +162,9 @@ def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
     if lens is not None and (lens.dtype != torch.int32 or tuple(lens.shape) != (n_slots, n_seqs) or
                              not lens.is_contiguous()):
         raise ValueError("lens must be a contiguous int32 (n_slots, n_seqs) tensor")
+    for t in (v, k_exp, v_exp, lens):
+        if t is not None and t.device != k.device:
+            raise ValueError(f"an 8-bit cache's tensors must share a device: {k.device} vs {t.device}")
     c = _abi.wfd_q8_cache()
     c.k, c.v, c.k_exp, c.v_exp, c.lens = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), rt.ptr(lens)
     c.n_slots, c.n_seqs, c.max_seq, c.n_kv_heads, c.head_dim = n_slots, n_seqs, max_seq, Hkv, Dh

@@ -108,6 +108,8 @@ def reserve_workspace(device: torch.device, max_items: int, head_dim: int = 128)
 
 
 def error_word(device: torch.device) -> torch.Tensor:
+    if device.type != "cuda":   # a host address would become the error word of the current GPU's kernels
+        raise ValueError(f"wavefront kernels run on CUDA devices only (no CPU path), got {device}")
     idx = device.index if device.index is not None else torch.cuda.current_device()
     with _state_lock:
         e = _err.get(idx)
