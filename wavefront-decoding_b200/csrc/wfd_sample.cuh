@@ -41,6 +41,7 @@
 #include <cooperative_groups.h>
 
 #include "wfd_model.cuh"
+#include "wfd_sample_bins.cuh"
 
 namespace wfd {
 
@@ -643,38 +644,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
       least = threshold(0, b, before, (unsigned long long)k);
     }
     if (use_p) {
-      // bounds of the mass up to each bin: its weights lie in [wl, wh]
+      // the bins in which the mass can cross top-p
       const float g = scale > 0.f ? 1.4426950408889634f / (scale * Tf) : 0.f;  // log2 weight of one bin
-      const double low = D < INF ? 0.9999 : 0.0;  // D = inf: no steps, any bin holds any weight
-      double lo = 0.0, hi = 0.0, wl[PER], wh[PER];
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const int b = tid * PER + e;
-        wh[e] = c[e] ? (double)c[e] * (double)exp2f(-g * fmaxf((float)b - 0.5f, 0.f)) * 1.0001 : 0.0;
-        wl[e] = c[e] ? (double)c[e] * (double)exp2f(-g * ((float)b + 0.5f)) * low : 0.0;
-        lo += wl[e];
-        hi += wh[e];
-      }
-      // prefix sums as integers (2^30 per unit, rounded outwards) so that the scan above serves
+      const SampleBounds<PER> bd = sample_bounds(c, tid * PER, g, D < INF ? 0.9999 : 0.0);
       unsigned long long tl, th, pl, ph;
-      const double F = 1073741824.0;
-      sample_scan2((unsigned long long)(lo * F), (unsigned long long)(hi * F) + 1, pl, ph, tl, th, s);
+      sample_scan2(bd.lo_sum, bd.hi_sum, pl, ph, tl, th, s);
       __syncthreads();
       if (tid == 0) s.bc[2] = s.bc[3] = kSampleBins - 1;
       __syncthreads();
-      // the first bins at which the upper and the lower sum reach these (the sums only
-      // grow: one bin each, or none)
-      const double slack = (double)kSampleThreads;  // more than the rounding of the terms above
-      const double first = (double)tp * (double)tl - 2.0 * slack, last = (double)tp * ((double)th + slack);
-      double rl = (double)pl - slack, rh = (double)ph + slack;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const double nl = rl + wl[e] * F, nh = rh + wh[e] * F + 1.0;
-        if (nh >= first && (rh < first || tid * PER + e == 0)) s.bc[2] = tid * PER + e;
-        if (nl >= last && rl < last) s.bc[3] = tid * PER + e;
-        rl = nl;
-        rh = nh;
-      }
+      sample_bracket(bd, pl, ph, tl, th, tp, tid * PER, [&](int b) { s.bc[2] = b; }, [&](int b) { s.bc[3] = b; });
       __syncthreads();
       const int b0 = (int)s.bc[2], b1 = (int)s.bc[3];
       unsigned long long z[2];
