@@ -211,7 +211,7 @@ class QuantKVCache(SlotKVCache):
         rt.dtype_code(dtype)
         if lens is None:
             lens = torch.zeros(K.shape[:2], dtype=torch.int32, device=K.device)
-        self._c = _ops.q8_cache_struct(K, V, k_exp, v_exp, lens)
+        _ops.check_q8_cache(K, V, k_exp, v_exp, lens)
         Dh = K.shape[4]
         if Dh < 16 or Dh > 256 or Dh & (Dh - 1):
             raise ValueError(f"head_dim {Dh}: an 8-bit cache takes powers of two from 16 to 256")
@@ -223,9 +223,23 @@ class QuantKVCache(SlotKVCache):
     def nbytes(self) -> int:
         return self.K.numel() + self.V.numel() + self.k_exp.numel() + self.v_exp.numel()
 
+    def __getstate__(self):   # (pickle restores no float8 storage: codes travel as bytes)
+        return dict(self.__dict__, K=self.K.view(torch.uint8), V=self.V.view(torch.uint8))
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, K=state["K"].view(torch.float8_e4m3fn), V=state["V"].view(torch.float8_e4m3fn))
+
+    def _struct(self):
+        """The C view of the attributes as they are at this call: any of them may have been replaced."""
+        if self.K.shape != (self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim):
+            raise ValueError(f"K is {tuple(self.K.shape)}, the cache was made with "
+                             f"{(self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim)}")
+        return _ops.q8_cache_struct(self.K, self.V, self.k_exp, self.v_exp, self.lens)
+
     def _call(self, name: str, *args) -> None:
-        rt.require_cuda(self.K)
-        rt.call(self.device, name, ctypes.byref(self._c), *args, rt.error_word(self.device).data_ptr(),
+        if rt.require_cuda(self.K) != self.device:
+            raise ValueError(f"K on {self.K.device}, cache on {self.device}")
+        rt.call(self.device, name, ctypes.byref(self._struct()), *args, rt.error_word(self.device).data_ptr(),
                 self._stream())
 
     def _rows(self, k, v, lead: tuple):
@@ -332,6 +346,6 @@ class QuantKVCache(SlotKVCache):
         if rt.require_cuda(q) != self.device:
             raise ValueError(f"rows on {q.device}, cache on {self.device}")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        _ops.wave_attn_q8_launch(self._c, q, k_new, v_new, items, int(max_q), int(slot_offset), None, int(kernel),
+        _ops.wave_attn_q8_launch(self._struct(), q, k_new, v_new, items, int(max_q), int(slot_offset), None, int(kernel),
                                  row_pos, out)
         return out

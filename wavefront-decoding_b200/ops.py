@@ -149,8 +149,8 @@ def plain_eager(t: torch.Tensor) -> bool:
     return type(t) is torch.Tensor and torch._C._len_torch_dispatch_stack() == 0 and not torch.compiler.is_compiling()
 
 
-def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
-    """The C view of an 8-bit cache's tensors, after the checks of their shapes, types and devices."""
+def check_q8_cache(k, v, k_exp, v_exp, lens) -> None:
+    """The shapes, types and devices of an 8-bit cache's tensors."""
     if k.dim() != 5 or v.shape != k.shape or k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or \
             not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("K, V must be contiguous float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) tensors")
@@ -165,6 +165,12 @@ def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
     for t in (v, k_exp, v_exp, lens):
         if t is not None and t.device != k.device:
             raise ValueError(f"an 8-bit cache's tensors must share a device: {k.device} vs {t.device}")
+
+
+def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
+    """The C view of an 8-bit cache's tensors as they are now, after their checks."""
+    check_q8_cache(k, v, k_exp, v_exp, lens)
+    n_slots, n_seqs, max_seq, Hkv, Dh = k.shape
     c = _abi.wfd_q8_cache()
     c.k, c.v, c.k_exp, c.v_exp, c.lens = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), rt.ptr(lens)
     c.n_slots, c.n_seqs, c.max_seq, c.n_kv_heads, c.head_dim = n_slots, n_seqs, max_seq, Hkv, Dh
