@@ -312,7 +312,8 @@ class QuantKVCache(SlotKVCache):
     def commit_window(self, items: torch.Tensor, *, accept_len: torch.Tensor | None = None,
                       accept_mask: torch.Tensor | None = None, slot_offset: int = 0, n_rows: int | None = None,
                       out: tuple[torch.Tensor, torch.Tensor] | None = None):
-        """SlotKVCache.commit_window: accepted rows move as they are, codes and exponents."""
+        """SlotKVCache.commit_window: accepted rows move as they are, codes and exponents (torch.ops.wfd.commit_q8)."""
+        rt.require_cuda(self.K)
         if (accept_len is None) == (accept_mask is None):
             raise ValueError("give exactly one of accept_len / accept_mask")
         items = _ops.i32(items, self.device).reshape(-1, 5)
@@ -321,31 +322,18 @@ class QuantKVCache(SlotKVCache):
         am = None
         if accept_mask is not None:
             am = torch.as_tensor(accept_mask).to(device=self.device, dtype=torch.uint8).contiguous()
-        if out is None:
-            if n_rows is None:
-                n_rows = int((items[:, 4] + items[:, 3]).max().item()) if n else 0
-            out = (torch.full((int(n_rows),), -1, dtype=torch.int32, device=self.device),
-                   torch.zeros(n, dtype=torch.int32, device=self.device))
-        acc_rows, acc_count = out
-        for t in out:
-            if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
-                raise ValueError("acc_rows / acc_count must be contiguous int32 tensors on the cache's device")
-        if acc_count.numel() < n or (al is not None and al.numel() < n):
-            raise ValueError("acc_count and accept_len need one entry per item")
-        rows = acc_rows.numel() if am is None else min(acc_rows.numel(), am.numel())
-        self._call("wfd_commit_window_q8", items.data_ptr(), n, rt.ptr(al), rt.ptr(am), acc_rows.data_ptr(),
-                   acc_count.data_ptr(), rows, int(slot_offset))
-        return (acc_rows if n_rows is None else acc_rows[:n_rows]), acc_count[:n]
+        cache = (self.K, self.V, self.k_exp, self.v_exp, self.lens)
+        if out is not None:
+            acc_rows, acc_count = out
+            torch.ops.wfd.commit_q8_out(*cache, items, al, am, int(slot_offset), acc_rows, acc_count)
+            return (acc_rows if n_rows is None else acc_rows[:n_rows]), acc_count[:n]
+        if n_rows is None:
+            n_rows = int((items[:, 4] + items[:, 3]).max().item()) if n else 0
+        return torch.ops.wfd.commit_q8(*cache, items, al, am, int(slot_offset), int(n_rows))
 
     def wave_attn(self, q, k_new, v_new, items, max_q: int, *, slot_offset: int = 0, out=None, kernel: int = -1,
                   update_lens: bool = True, row_pos=None):
         """Fused quantising append + wavefront attention over this cache's slots (attention.wave_attn_q8)."""
-        if not update_lens:
-            return _attn.wave_attn_q8(q, k_new, v_new, self.K, self.V, self.k_exp, self.v_exp, items, max_q,
-                                      slot_offset=slot_offset, out=out, kernel=kernel, row_pos=row_pos)
-        if rt.require_cuda(q) != self.device:
-            raise ValueError(f"rows on {q.device}, cache on {self.device}")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        _ops.wave_attn_q8_launch(self._struct(), q, k_new, v_new, items, int(max_q), int(slot_offset), None, int(kernel),
-                                 row_pos, out)
-        return out
+        return _attn.wave_attn_q8(q, k_new, v_new, self.K, self.V, self.k_exp, self.v_exp, items, max_q,
+                                  lens=self.lens if update_lens else None, slot_offset=slot_offset, out=out,
+                                  kernel=kernel, row_pos=row_pos)

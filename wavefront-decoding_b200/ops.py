@@ -35,6 +35,10 @@ dispatcher.
       wave_attn over an 8-bit cache (kv_cache.QuantKVCache): the window rows are
       quantised into it, and every key is attended as the cache holds it.
   wfd::wave_attn_q8_out(..., Tensor(f!) out) -> ()
+  wfd::commit_q8(k_cache!, v_cache!, k_exp!, v_exp!, lens!, items, accept_len?,
+                 accept_mask?, slot_offset, n_rows) -> (acc_rows, acc_count)
+  wfd::commit_q8_out(..., Tensor(f!) acc_rows, Tensor(g!) acc_count) -> ()
+      commit of verify windows in an 8-bit cache: codes and exponents move as they are.
 """
 from __future__ import annotations
 
@@ -72,6 +76,12 @@ _SCHEMAS = {
                         "Tensor(b!) v_cache, Tensor(c!) k_exp, Tensor(d!) v_exp, Tensor items, int max_q, "
                         "Tensor(e!)? lens, int slot_offset, float? scale, int kernel, Tensor? row_pos, "
                         "Tensor(f!) out) -> ()",
+    "commit_q8": "commit_q8(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_exp, Tensor(d!) v_exp, "
+                 "Tensor(e!) lens, Tensor items, Tensor? accept_len, Tensor? accept_mask, int slot_offset, int n_rows) "
+                 "-> (Tensor, Tensor)",
+    "commit_q8_out": "commit_q8_out(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_exp, Tensor(d!) v_exp, "
+                     "Tensor(e!) lens, Tensor items, Tensor? accept_len, Tensor? accept_mask, int slot_offset, "
+                     "Tensor(f!) acc_rows, Tensor(g!) acc_count) -> ()",
 }
 for _schema in _SCHEMAS.values():
     _LIB.define(_schema)
@@ -327,6 +337,33 @@ def _wave_attn_q8_cuda(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, m
     return out
 
 
+def _commit_q8_out_cuda(k_cache, v_cache, k_exp, v_exp, lens, items, accept_len, accept_mask, slot_offset, acc_rows,
+                        acc_count):
+    dev = _check_commit(k_cache, v_cache, lens, items, accept_len, accept_mask)
+    n = items.shape[0]
+    for t in (acc_rows, acc_count):
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise ValueError("acc_rows / acc_count must be contiguous int32 tensors on the cache's device")
+    if acc_count.numel() < n or (accept_len is not None and accept_len.numel() < n):
+        raise ValueError("acc_count and accept_len need one entry per item")
+    c = q8_cache_struct(k_cache, v_cache, k_exp, v_exp, lens)
+    al = None if accept_len is None else accept_len.contiguous()
+    am = None if accept_mask is None else accept_mask.contiguous()
+    # q rows both row-indexed arrays cover: the kernel skips (and reports) windows past them
+    n_rows = acc_rows.numel() if am is None else min(acc_rows.numel(), am.numel())
+    rt.call(dev, "wfd_commit_window_q8", ctypes.byref(c), items.data_ptr(), n, rt.ptr(al), rt.ptr(am),
+            acc_rows.data_ptr(), acc_count.data_ptr(), n_rows, int(slot_offset), rt.error_word(dev).data_ptr(),
+            rt.stream_ptr(dev))
+
+
+def _commit_q8_cuda(k_cache, v_cache, k_exp, v_exp, lens, items, accept_len, accept_mask, slot_offset, n_rows):
+    acc_rows = torch.full((int(n_rows),), -1, dtype=torch.int32, device=k_cache.device)
+    acc_count = torch.zeros((items.shape[0],), dtype=torch.int32, device=k_cache.device)
+    _commit_q8_out_cuda(k_cache, v_cache, k_exp, v_exp, lens, items, accept_len, accept_mask, slot_offset, acc_rows,
+                        acc_count)
+    return acc_rows, acc_count
+
+
 _LIB.impl("attn", _attn_cuda, "CUDA")
 _LIB.impl("attn_out", _attn_out_cuda, "CUDA")
 _LIB.impl("wave_attn", _wave_attn_cuda, "CUDA")
@@ -336,6 +373,8 @@ _LIB.impl("commit_out", _commit_out_cuda, "CUDA")
 _LIB.impl("commit_drop", _commit_drop_cuda, "CUDA")
 _LIB.impl("wave_attn_q8", _wave_attn_q8_cuda, "CUDA")
 _LIB.impl("wave_attn_q8_out", _wave_attn_q8_out_cuda, "CUDA")
+_LIB.impl("commit_q8", _commit_q8_cuda, "CUDA")
+_LIB.impl("commit_q8_out", _commit_q8_out_cuda, "CUDA")
 
 
 # ---------------------------------------------------------------------------
@@ -387,4 +426,15 @@ def _wave_attn_q8_fake(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, m
 @torch.library.register_fake("wfd::wave_attn_q8_out")
 def _wave_attn_q8_out_fake(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q, lens, slot_offset, scale,
                            kernel, row_pos, out):
+    return None
+
+
+@torch.library.register_fake("wfd::commit_q8")
+def _commit_q8_fake(k_cache, v_cache, k_exp, v_exp, lens, items, accept_len, accept_mask, slot_offset, n_rows):
+    return (lens.new_empty((n_rows,)), lens.new_empty((items.shape[0],)))
+
+
+@torch.library.register_fake("wfd::commit_q8_out")
+def _commit_q8_out_fake(k_cache, v_cache, k_exp, v_exp, lens, items, accept_len, accept_mask, slot_offset, acc_rows,
+                        acc_count):
     return None
