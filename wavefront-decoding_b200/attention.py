@@ -207,7 +207,7 @@ def wave_attn_q8(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q: 
         rt.require_cuda(q)
     args = (q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, int(max_q), lens, int(slot_offset), scale,
             int(kernel), row_pos)
-    if _ops.plain_eager(q):   # nothing traces or dispatches on the call: the op's kernel without the dispatcher (11 us)
+    if _ops.plain_eager((q, k_new, v_new, out), (k_cache, v_cache, k_exp, v_exp, items, lens, row_pos)):   # nothing traces or dispatches on the call: the op's kernel without the dispatcher (11 us)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
         _ops._wave_attn_q8_out_cuda(*args, out)
         return out

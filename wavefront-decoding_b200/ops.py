@@ -46,6 +46,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 from . import runtime as rt
@@ -154,9 +155,24 @@ def _check_commit(k_cache, v_cache, lens, items, accept_len, accept_mask):
     return dev
 
 
-def plain_eager(t: torch.Tensor) -> bool:
-    """Whether a call on t can go to the kernel without the dispatcher: a plain tensor, nothing compiling or tracing."""
-    return type(t) is torch.Tensor and torch._C._len_torch_dispatch_stack() == 0 and not torch.compiler.is_compiling()
+def plain_eager(rows, others) -> bool:
+    """Whether a call on these tensors can go to the kernel without the dispatcher, because the dispatcher would only
+    hand it on: nothing compiles, traces, transforms (vmap, grad, jvp), intercepts or profiles, and every tensor is a
+    plain one that needs no gradient; those of `rows` (whose type may be float32) are no views that negate.  None: an
+    argument not given."""
+    if torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack() or \
+            torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None or \
+            forward_ad._current_level >= 0 or torch.autograd._profiler_enabled() or \
+            torch._C._get_tracing_state() is not None:
+        return False
+    for t in rows:
+        if t is not None and (type(t) is not torch.Tensor or t.requires_grad or t.is_neg() or
+                              torch._is_functional_tensor(t)):
+            return False
+    for t in others:
+        if t is not None and (type(t) is not torch.Tensor or t.requires_grad):
+            return False
+    return True
 
 
 def check_q8_cache(k, v, k_exp, v_exp, lens) -> None:
