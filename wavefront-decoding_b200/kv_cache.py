@@ -231,14 +231,14 @@ class QuantKVCache(SlotKVCache):
 
     def _struct(self):
         """The C view of the attributes as they are at this call: any of them may have been replaced."""
-        if self.K.shape != (self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim):
-            raise ValueError(f"K is {tuple(self.K.shape)}, the cache was made with "
-                             f"{(self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim)}")
+        shape = (self.n_slots, self.B, self.S, self.n_kv_head, self.head_dim)
+        if self.K.shape != shape or self.K.device != self.device:
+            raise ValueError(f"K is {tuple(self.K.shape)} on {self.K.device}, the cache was made with {shape} on "
+                             f"{self.device}")
         return _ops.q8_cache_struct(self.K, self.V, self.k_exp, self.v_exp, self.lens)
 
     def _call(self, name: str, *args) -> None:
-        if rt.require_cuda(self.K) != self.device:
-            raise ValueError(f"K on {self.K.device}, cache on {self.device}")
+        rt.require_cuda(self.K)
         rt.call(self.device, name, ctypes.byref(self._struct()), *args, rt.error_word(self.device).data_ptr(),
                 self._stream())
 
@@ -272,11 +272,11 @@ class QuantKVCache(SlotKVCache):
         if not sl.numel() == sq.numel() == ps.numel() == n:
             raise ValueError(f"{n} rows need {n} slots, seq_ids and positions")
         k, v, dt = self._rows(k, v, (n,))
-        step = _abi.WFD_Q8_MAX_APPEND
+        step, row = _abi.WFD_Q8_MAX_APPEND, self.n_kv_head * self.head_dim * k.element_size()
+        pk, pv, *idx = (t.data_ptr() for t in (k, v, sl, sq, ps))
         for i in range(0, n, step):
-            m = min(step, n - i)
-            self._call("wfd_append_q8", k[i:].data_ptr(), v[i:].data_ptr(), sl[i:].data_ptr(), sq[i:].data_ptr(),
-                       ps[i:].data_ptr(), m, int(slot_offset), dt)
+            self._call("wfd_append_q8", pk + i * row, pv + i * row, *(p + 4 * i for p in idx), min(step, n - i),
+                       int(slot_offset), dt)
 
     def gather_packed(self, slots: torch.Tensor, seq_ids: torch.Tensor, cu_k: torch.Tensor, total: int, *, out=None):
         """Read back: segment i holds the values of positions [0, cu_k[i+1] -

@@ -177,29 +177,30 @@ def plain_eager(rows, others) -> bool:
 
 def check_q8_cache(k, v, k_exp, v_exp, lens) -> None:
     """The shapes, types and devices of an 8-bit cache's tensors."""
-    if k.dim() != 5 or v.shape != k.shape or k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or \
+    shape = k.shape
+    if len(shape) != 5 or v.shape != shape or k.dtype is not torch.float8_e4m3fn or v.dtype is not k.dtype or \
             not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("K, V must be contiguous float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) tensors")
-    n_slots, n_seqs, max_seq, Hkv, Dh = k.shape
+    n_slots, n_seqs, max_seq, Hkv, _ = shape
     want = (n_slots, n_seqs, Hkv, max_seq)
     for e in (k_exp, v_exp):
-        if e.dtype != torch.int8 or tuple(e.shape) != want or not e.is_contiguous():
+        if e.dtype is not torch.int8 or e.shape != want or not e.is_contiguous():
             raise ValueError("k_exp, v_exp must be contiguous int8 (n_slots, n_seqs, Hkv, max_seq) tensors")
-    if lens is not None and (lens.dtype != torch.int32 or tuple(lens.shape) != (n_slots, n_seqs) or
+    if lens is not None and (lens.dtype is not torch.int32 or lens.shape != (n_slots, n_seqs) or
                              not lens.is_contiguous()):
         raise ValueError("lens must be a contiguous int32 (n_slots, n_seqs) tensor")
+    at = k.get_device() if k.is_cuda else None     # (an index compares faster than a device)
     for t in (v, k_exp, v_exp, lens):
-        if t is not None and t.device != k.device:
+        if t is not None and (t.device != k.device if at is None else t.get_device() != at):
             raise ValueError(f"an 8-bit cache's tensors must share a device: {k.device} vs {t.device}")
 
 
 def q8_cache_struct(k, v, k_exp, v_exp, lens) -> "_abi.wfd_q8_cache":
     """The C view of an 8-bit cache's tensors as they are now, after their checks."""
     check_q8_cache(k, v, k_exp, v_exp, lens)
-    n_slots, n_seqs, max_seq, Hkv, Dh = k.shape
     c = _abi.wfd_q8_cache()
     c.k, c.v, c.k_exp, c.v_exp, c.lens = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), rt.ptr(lens)
-    c.n_slots, c.n_seqs, c.max_seq, c.n_kv_heads, c.head_dim = n_slots, n_seqs, max_seq, Hkv, Dh
+    c.n_slots, c.n_seqs, c.max_seq, c.n_kv_heads, c.head_dim = k.shape
     return c
 
 
