@@ -476,6 +476,12 @@ typedef struct wfd_sample_params {
 } wfd_sample_params;
 
 int wfd_sample_rows(const wfd_sample_params* p, void* stream);
+/* wfd_sample_rows where the RMSNorm before the product whose output x is has been
+ * folded into its weight (as wfd_rope_split_norm): xn are the rows (n, d; row stride
+ * ldx) that the product took, of x's type, 16-byte aligned, d and ldx multiples of 8.
+ * The logits are x_i / sqrt(mean(xn[r]^2) + eps); T <= 0 gives the first maximum of x
+ * itself, what wfd_argmax_rows finds. */
+int wfd_sample_rows_norm(const wfd_sample_params* p, const void* xn, int32_t ldx, int32_t d, float eps, void* stream);
 /* sizeof(wfd_sample_params) as compiled into the library. */
 size_t wfd_sample_params_bytes(void);
 

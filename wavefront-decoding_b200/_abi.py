@@ -31,7 +31,7 @@ EXPORTED = (
     "wfd_linear", "wfd_linear_params_bytes", "wfd_rope_split_norm", "wfd_silu_mul_norm",
     "wfd_q8_cache_bytes", "wfd_append_q8", "wfd_write_prefill_q8", "wfd_gather_q8", "wfd_commit_window_q8",
     "wfd_wave_attn_q8", "wfd_wave_attn_q8_workspace",
-    "wfd_sample_rows", "wfd_sample_params_bytes",
+    "wfd_sample_rows", "wfd_sample_rows_norm", "wfd_sample_params_bytes",
 )
 WFD_Q8_MAX_APPEND = 16384
 
@@ -167,6 +167,8 @@ _SIGS = {
     "wfd_wave_attn_q8": ([_I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _F, _P, _S, _P, _P], _I),
     # const wfd_sample_params*, stream
     "wfd_sample_rows": ([_P, _P], _I),
+    # const wfd_sample_params*, normalised rows, their stride, d, eps, stream
+    "wfd_sample_rows_norm": ([_P, _P, _I, _I, _F, _P], _I),
     "wfd_sample_params_bytes": ([], _S),
     # const wfd_sched_params*, stream
     "wfd_sched_pre_tick": ([_P, _P], _I),

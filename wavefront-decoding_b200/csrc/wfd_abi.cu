@@ -1683,11 +1683,8 @@ int launch_sample(const SampleParams& p, int cluster, size_t smem, cudaStream_t 
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, p) == cudaSuccess ? WFD_OK : WFD_ERR_CUDA;
 }
-}  // namespace
 
-extern "C" size_t wfd_sample_params_bytes(void) { return sizeof(wfd_sample_params); }
-
-extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
+int sample_rows(const wfd_sample_params* a, const void* xn, int xn_ld, int xn_d, float eps, void* stream) {
   if (!a || a->n < 0 || a->V <= 0 || a->V > kSampleMaxV || a->ldx < a->V) return WFD_ERR_INVALID_ARG;
   if (a->dtype != WFD_DTYPE_BF16 && a->dtype != WFD_DTYPE_F32) return WFD_ERR_UNSUPPORTED;
   if (a->n == 0) return WFD_OK;
@@ -1720,6 +1717,10 @@ extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
   p.u_cols = a->u_cols;
   p.seq_stride = a->seq_stride;
   p.pos_stride = a->pos_stride;
+  p.norm_x = xn;
+  p.norm_ld = xn_ld;
+  p.norm_d = xn_d;
+  p.norm_eps = eps;
   // CTAs per row: as many as fit at two CTAs an SM, with at least a tile of tokens
   // each; and more, up to 8, where that lets a slice fit in half an SM's shared memory
   int cluster = 1;
@@ -1737,4 +1738,18 @@ extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return a->dtype == WFD_DTYPE_BF16 ? launch_sample<__nv_bfloat16>(p, cluster, smem, st)
                                     : launch_sample<float>(p, cluster, smem, st);
+}
+}  // namespace
+
+extern "C" size_t wfd_sample_params_bytes(void) { return sizeof(wfd_sample_params); }
+
+extern "C" int wfd_sample_rows(const wfd_sample_params* a, void* stream) {
+  return sample_rows(a, nullptr, 0, 0, 0.f, stream);
+}
+
+extern "C" int wfd_sample_rows_norm(const wfd_sample_params* a, const void* xn, int32_t ldx, int32_t d, float eps,
+                                    void* stream) {
+  if (!a || a->n < 0) return WFD_ERR_INVALID_ARG;
+  if (a->n > 0 && !norm_args_ok(xn, ldx, d, eps)) return xn && !aligned16(xn) ? WFD_ERR_ALIGNMENT : WFD_ERR_INVALID_ARG;
+  return sample_rows(a, xn, ldx, d, eps, stream);
 }

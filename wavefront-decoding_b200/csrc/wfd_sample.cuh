@@ -70,6 +70,9 @@ struct SampleParams {
   long long ldx;
   int n, V, vec;  // vec: 16-byte loads are aligned
   int n_params, u_stride, u_cols, seq_stride, pos_stride;
+  const void* norm_x;  // rows whose RMS divides the logits, or null
+  int norm_ld, norm_d;
+  float norm_eps;
   int slice;  // tokens per CTA of a row's cluster, a multiple of kSampleTile
   int cached; // the slice is kept in shared memory
 };
@@ -257,11 +260,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     }
     return;
   }
-  const float Tf = p.temperature != nullptr ? p.temperature[pr] : 1.f;
+  float Tf = p.temperature != nullptr ? p.temperature[pr] : 1.f;
   const float uf = p.u[(long long)pr * p.u_stride + pc];
   const int k = p.top_k != nullptr ? p.top_k[pr] : 0;
   const float tp = p.top_p != nullptr ? p.top_p[pr] : 1.f;
   const double minp = p.min_p != nullptr ? fmin((double)p.min_p[pr], 1.0) : 0.0;
+
+  // Logits x_i / rms: the row's RMS goes into the temperature, and so leaves the order of
+  // its tokens alone.  Every CTA of the row sums it in the same order.
+  if (p.norm_x != nullptr) {
+    const T* nx = static_cast<const T*>(p.norm_x) + (long long)r * p.norm_ld;
+    float ss = 0.f;
+    for (int c = tid * 8; c < p.norm_d; c += kSampleThreads * 8) {
+      float v[8];
+      Vec8<T>::load(nx + c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) s.part[2][warp] = __float_as_uint(ss);
+    __syncthreads();
+    float tot = 0.f;
+    for (int w = 0; w < kSampleWarps; ++w) tot += __uint_as_float((uint32_t)s.part[2][w]);
+    if (Tf > 0.f) Tf = fmaxf(Tf * sqrtf(tot / (float)p.norm_d + p.norm_eps), 1e-45f);
+  }
 
   SampleRow<T> row;
   row.x = static_cast<const T*>(p.x) + (long long)r * p.ldx;

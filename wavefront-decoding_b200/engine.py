@@ -141,9 +141,9 @@ class _Sampler:
         for dst, v in vals:
             dst[:self.B].copy_(v)
 
-    def draw(self, logits: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None):
+    def draw(self, logits: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None, **norm):
         return fused.sample_rows(logits, self.u, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p,
-                                 min_p=self.min_p, row_seq=seq, row_pos=pos, out=out)
+                                 min_p=self.min_p, row_seq=seq, row_pos=pos, out=out, **norm)
 
 
 class WaveEngine:
@@ -234,9 +234,6 @@ class WaveEngine:
             for (kind, _), t in self._tables.items():
                 if kind == "C":
                     t.graph = None
-            # the sampled C body runs the final RMSNorm that the folded greedy one leaves out
-            if self.model.fold_norms:
-                self._launches["C"] += 1 if self.sampling else -1
 
     @torch.no_grad()
     def first_ids(self, logits: torch.Tensor, prompt_len: int) -> list[int]:
@@ -361,7 +358,8 @@ class WaveEngine:
             for j, blk in enumerate(m.coda):
                 x = self._segment_block(blk, x, t, cfg.slot_coda(j))
             if self.sampling:
-                self._sampler.draw(m.head(x), tab[:, 3], tab[:, 1], t.out)
+                logits, norm = m.unscaled_head(x)
+                self._sampler.draw(logits, tab[:, 3], tab[:, 1], t.out, **norm)
             else:
                 m.greedy_ids(x, t.out)
 

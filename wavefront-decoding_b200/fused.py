@@ -160,7 +160,8 @@ def argmax_rows(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 def sample_rows(x: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | None = None,
                 top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
                 min_p: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
-                row_pos: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                row_pos: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                norm_x: torch.Tensor | None = None, norm_eps: float = 0.0) -> torch.Tensor:
     """Sampled ids (int32, one per row) of logits x (n, V), bf16 or fp32 (padded rows,
     x.stride(0) > V, are read in place).
 
@@ -175,8 +176,11 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     temperature, top_p, min_p: fp32, top_k: int32, one entry per row, or None (1, no
     filter).  u: fp32 numbers in [0, 1), one per row.  With row_seq (int32, any
     stride) row r takes entry row_seq[r] of these vectors instead, and with row_pos
-    u is (entries, columns) and row r takes u[entry, row_pos[r]]."""
-    dev = rt.require_cuda(x, u, temperature, top_k, top_p, min_p, row_seq, row_pos, out)
+    u is (entries, columns) and row r takes u[entry, row_pos[r]].  norm_x (n, d): the
+    rows the lm_head product read when the final RMSNorm is folded into its weight
+    (fold_norm); the logits are then x over each row's RMS, and temperature <= 0
+    gives what argmax_rows finds in x."""
+    dev = rt.require_cuda(x, u, temperature, top_k, top_p, min_p, row_seq, row_pos, out, norm_x)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"sample_rows: x must be (n, V) rows, got {tuple(x.shape)}")
     n, V = x.shape
@@ -211,7 +215,12 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     p.n_params = entries
     p.u_cols = 1 if u.dim() == 1 else u.shape[1]
     p.u_stride = max(p.u_cols, u.stride(0))
-    rt.call(dev, "wfd_sample_rows", ctypes.byref(p), rt.stream_ptr(dev))
+    if norm_x is None:
+        rt.call(dev, "wfd_sample_rows", ctypes.byref(p), rt.stream_ptr(dev))
+        return out
+    if norm_x.dtype != x.dtype:
+        raise TypeError("sample_rows: norm_x must have x's type")
+    rt.call(dev, "wfd_sample_rows_norm", ctypes.byref(p), *_norm_rows(norm_x, n), float(norm_eps), rt.stream_ptr(dev))
     return out
 
 

@@ -212,9 +212,15 @@ class LoopedLM:
         """out (int32) = argmax of each row's logits (first maximum), without an fp32 copy.
         With folded norms the final RMSNorm's weight sits in lm_head_n and its row
         scale, positive, leaves the argmax unchanged: it is not computed."""
+        return fused.argmax_rows(self.unscaled_head(x)[0], out)
+
+    def unscaled_head(self, x: torch.Tensor) -> tuple[torch.Tensor, dict]:
+        """The product that ids are taken from, greedy and drawn ones alike, and what makes logits of it
+        (fused.sample_rows): with folded norms each row still lacks its final RMSNorm's scale."""
+        x = x.contiguous()
         if self.fold_norms:
-            return fused.argmax_rows(x.contiguous() @ self.lm_head_n, out)
-        return fused.argmax_rows(self.rmsnorm(x.contiguous(), self.final_norm) @ self.lm_head, out)
+            return x @ self.lm_head_n, {"norm_x": x, "norm_eps": self.cfg.norm_eps}
+        return self.head(x), {}
 
     # ------------------------------------------------------------------
     @torch.no_grad()
