@@ -217,19 +217,27 @@ class DeviceWave:
                         self._tick(p)
             ticks += k
         torch.cuda.synchronize(self.device)
-        rt.read_device_error(self.device)
+        error = None
+        try:
+            rt.read_device_error(self.device)
+        except _abi.WfdError as err:
+            error = err
         bt.walltime_s = time.perf_counter() - t0
         self.ticks_replayed = ticks
 
         committed = self.committed.cpu()
         seq_ct = self.seq_ct.cpu()
         n_commit = self.n_commit.cpu()
+        tokens = [committed[b, :min(int(n_commit[b]), self.max_new)].tolist() for b in range(B)]
+        e.drawn([min(ts, default=0) for ts in tokens], range(B))   # (before the error that the gather of such an id reports)
+        if error is not None:
+            raise error
         bc = self.batch_ct.tolist()
         bt.n_r_calls, bt.n_p_calls, bt.n_c_calls = bc[0], bc[1], bc[2]
         bt.r_union_total, bt.r_union_max = bc[3], bc[4]
         for b in range(B):
             tr = GenerationTrace()
-            tr.tokens = committed[b, :min(int(n_commit[b]), self.max_new)].tolist()
+            tr.tokens = tokens[b]
             for i, name in enumerate(_CT):
                 setattr(tr, name, int(seq_ct[b, i]))
             tr.walltime_s = bt.walltime_s

@@ -107,7 +107,9 @@ class SamplingParams:
     alike.  A draft is then accepted iff it is the token that full depth draws, so
     wavefront and draft-then-verify decoding commit the tokens that sequential
     decoding draws from the same numbers, as they do greedily.  temperature (<= 0:
-    greedy), top_k (0: all), top_p and min_p: one value, or one per sequence."""
+    the ids of greedy decoding), top_k (0: all), top_p and min_p: one value, or one
+    per sequence.  A generation that meets a row whose logits are all -inf or NaN
+    ends with an error."""
     u: torch.Tensor
     temperature: float | torch.Tensor = 1.0
     top_k: int | torch.Tensor = 0
@@ -241,7 +243,14 @@ class WaveEngine:
         if not self.sampling:
             return logits.argmax(dim=-1).tolist()
         seq = torch.arange(self.B, dtype=torch.int32, device=self.device)
-        return self._sampler.draw(logits, seq, torch.full_like(seq, prompt_len - 1)).tolist()
+        return self.drawn(self._sampler.draw(logits, seq, torch.full_like(seq, prompt_len - 1)).tolist(), range(self.B))
+
+    def drawn(self, ids: list[int], seq_ids) -> list[int]:
+        """The ids, unless sampling has left one out (fused.sample_rows gives -1 where no logit is above -inf)."""
+        if self.sampling and min(ids, default=0) < 0:
+            lost = sorted({int(b) for b, i in zip(seq_ids, ids) if i < 0})
+            raise RuntimeError(f"no token to draw: every logit is -inf or NaN (sequences {lost})")
+        return ids
 
     def drop_positions_at_and_after(self, b: int, position: int) -> None:
         self.cache.drop_positions_at_and_after(b, position)
@@ -424,7 +433,7 @@ class WaveEngine:
         t = self._fill("C", toks, seq_ids, [tk.hidden for tk in toks])
         self._run("C", t)
         self.d2h_bytes += 4 * len(toks)
-        return t.out[:len(toks)].tolist()
+        return self.drawn(t.out[:len(toks)].tolist(), seq_ids)
 
     # reporting
     @property
