@@ -444,8 +444,8 @@ int wfd_argmax_rows(const void* x, int32_t* out, int32_t n, int32_t V, int32_t d
  * ascending":
  *   top_k  keeps the first top_k tokens         (top_k <= 0 or >= V: all)
  *   top_p  of these, every token whose predecessors weigh less than top_p times
- *          all of them; the first in any case     (top_p >= 1: all)
- *   min_p  of these, w_i >= min_p                (min_p <= 0: all; > 1 counts as 1)
+ *          all of them; the first in any case     (top_p >= 1 or NaN: all)
+ *   min_p  of these, w_i >= min_p                (min_p <= 0: all; > 1 or NaN counts as 1)
  * and out[r] is the first index, in index order, at which the kept weight up to
  * and including it exceeds u times the kept weight (u < 0 or NaN counts as 0; u >= 1
  * gives the last kept token).  T <= 0 or NaN: the first index of the maximum.  A NaN

@@ -234,6 +234,27 @@ __device__ __forceinline__ void sample_scan2(unsigned long long a, unsigned long
   }
 }
 
+// Root mean square of a row of d values, in every thread; each CTA of a row sums in the
+// same order.
+template <typename T>
+__device__ __forceinline__ float sample_rms(const T* x, int d, float eps, SampleShared& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float ss = 0.f;
+  for (int c = threadIdx.x * 8; c < d; c += kSampleThreads * 8) {
+    float v[8];
+    Vec8<T>::load(x + c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (lane == 0) s.part[2][warp] = __float_as_uint(ss);
+  __syncthreads();
+  float tot = 0.f;
+  for (int w = 0; w < kSampleWarps; ++w) tot += __uint_as_float((uint32_t)s.part[2][w]);
+  return sqrtf(tot / (float)d + eps);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const SampleParams p) {
   namespace cg = cooperative_groups;
@@ -266,24 +287,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
   const float tp = p.top_p != nullptr ? p.top_p[pr] : 1.f;
   const double minp = p.min_p != nullptr ? fmin((double)p.min_p[pr], 1.0) : 0.0;
 
-  // Logits x_i / rms: the row's RMS goes into the temperature, and so leaves the order of
-  // its tokens alone.  Every CTA of the row sums it in the same order.
-  if (p.norm_x != nullptr) {
-    const T* nx = static_cast<const T*>(p.norm_x) + (long long)r * p.norm_ld;
-    float ss = 0.f;
-    for (int c = tid * 8; c < p.norm_d; c += kSampleThreads * 8) {
-      float v[8];
-      Vec8<T>::load(nx + c, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) s.part[2][warp] = __float_as_uint(ss);
-    __syncthreads();
-    float tot = 0.f;
-    for (int w = 0; w < kSampleWarps; ++w) tot += __uint_as_float((uint32_t)s.part[2][w]);
-    if (Tf > 0.f) Tf = fmaxf(Tf * sqrtf(tot / (float)p.norm_d + p.norm_eps), 1e-45f);
+  if (p.norm_x != nullptr) {  // logits x_i / rms: into the temperature, which leaves the order of the tokens alone
+    const float rms = sample_rms(static_cast<const T*>(p.norm_x) + (long long)r * p.norm_ld, p.norm_d, p.norm_eps, s);
+    if (Tf > 0.f) Tf = fmaxf(Tf * rms, 1e-45f);
   }
 
   SampleRow<T> row;
@@ -668,7 +674,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_rows_kernel(const Sa
     }
     if (use_p) {
       // the bins in which the mass can cross top-p
-      const float g = scale > 0.f ? 1.4426950408889634f / (scale * Tf) : 0.f;  // log2 weight of one bin
+      const float g = scale > 0.f ? (float)(weight.c / 32.0 / (double)scale) : 0.f;  // log2 weight of one bin
       const SampleBounds<PER> bd = sample_bounds(c, tid * PER, g, D < INF ? 0.9999 : 0.0);
       unsigned long long tl, th, pl, ph;
       sample_scan2(bd.lo_sum, bd.hi_sum, pl, ph, tl, th, s);
