@@ -193,7 +193,7 @@ def wave_attn_q8(q, k_new, v_new, k_cache, v_cache, k_exp, v_exp, items, max_q: 
                  row_pos: torch.Tensor | None = None):
     """wave_attn over an 8-bit slot cache (kv_cache.QuantKVCache): the dispatcher op
     torch.ops.wfd.wave_attn_q8 (wave_attn_q8_out with `out`), or its kernel directly
-    where no tracing or dispatch mode is active.
+    where the dispatcher would do nothing else (ops.plain_eager).
 
     k_cache / v_cache: float8_e4m3fn (n_slots, n_seqs, max_seq, Hkv, Dh) codes;
     k_exp / v_exp: int8 (n_slots, n_seqs, Hkv, max_seq); a cached value is code *

@@ -17,7 +17,7 @@
 // registers; more vectors are further units over the same keys.
 //
 // Bound by latency: 32 windows of 3 rows over 777 keys, 8 heads of 64, fp32, take
-// 28 us (4 us of HBM time), three units a CTA of three rounds of 256 keys, each
+// 30 us a call (4 us of HBM time), three units a CTA of three rounds of 256 keys, each
 // waiting for its loads, and a merge of 8 warps.  (Loads in branches, one round trip
 // each, and 12 warps that spilled: 41 us; scalar products instead of pairs: 30.)
 #pragma once

@@ -31,10 +31,10 @@
 // pass copies the slice to shared memory (where it fits), the later ones read it
 // there.  Only tokens that count are weighed: a lane takes its own in turn (weighing all of
 // them cost 28 thousand cycles a row of which 400 tokens weigh, this 7).  128 rows of
-// 50304 bf16 logits with temperatures of 0.5 to 1.5, top-k, top-p and min-p take 67 us,
-// one fp32 row of 32000 with top-p 19.7, 32 rows of 131071, half masked, 49: bound by the
+// 50304 bf16 logits with temperatures of 0.5 to 1.5, top-k, top-p and min-p take 66 us a call,
+// one fp32 row of 32000 with top-p 13 to 16, 32 rows of 131071, half masked, 51: bound by the
 // instructions of the exact pass where every token weighs (40 to 100 a token, an SM
-// issuing 54 % of its cycles), by the dependent passes and cluster barriers otherwise.
+// issuing 51 % of its cycles), by the dependent passes and cluster barriers otherwise.
 // (Eight independent weights at a time, the bins' masses in a loop of their own: 70 us.)
 #pragma once
 

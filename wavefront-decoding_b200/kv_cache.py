@@ -202,7 +202,8 @@ class QuantKVCache(SlotKVCache):
     @classmethod
     def wrap(cls, K: torch.Tensor, V: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
              lens: torch.Tensor | None = None, *, dtype: torch.dtype = torch.bfloat16) -> "QuantKVCache":
-        """Adopt existing code and exponent tensors without copying (every code finite)."""
+        """Adopt existing code and exponent tensors without copying (one device; every code finite, every exponent
+        from -32 to 32)."""
         self = cls.__new__(cls)
         self._adopt(K, V, k_exp, v_exp, lens, dtype)
         return self
